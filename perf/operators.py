@@ -112,7 +112,7 @@ def _key_rows(shape, g, dev):
 def _scale(amax, fmt):
     amax = amax.clamp(min=TINY)
     if fmt == "int8":
-        return amax / 127.0
+        return (amax.double() / 127.0).float()
     part, e = torch.frexp(amax)                                          # amax = part 2^e, part in [1/2, 1); 448 = 0.875 * 2^9
     return torch.ldexp(torch.ones_like(amax), e - 9 + (part > 0.875))
 
@@ -120,7 +120,7 @@ def _scale(amax, fmt):
 def _round_codes(x, s, fmt):
     if fmt == "e4m3":
         return (x * s.reciprocal()).to(torch.float8_e4m3fn)              # a power of two: the product is exact
-    return torch.round(x.double() * s.reciprocal().double()).to(torch.int8)
+    return torch.round(x.double() * s.double().reciprocal().float().double()).to(torch.int8)
 
 
 def _spread(s, cap):
