@@ -361,6 +361,61 @@ int t2s_gemm_wgrad_splits(int64_t rows, int n_out, int n_in);
 int t2s_gemm_wgrad(const void* dy, const void* x, float* dw, float* slabs, int64_t rows, int n_out, int n_in, int64_t ld_dy,
                    int64_t ld_x, int splits, int accumulate, t2s_stream_t stream);
 
+/* ---- answer decoding: an 8-bit key / value cache (vitxt_gqa_amd/csrc/kv8.hip) ---------------------------------------------------------
+ * The eval loop (pythia/models/t2s.py:315-354) attends, in every step, to the same prefix of up to 10 120 rows.  The cache holds keys
+ * and values of B sequences and H heads of 64 dims in 8 bits with one fp32 scale per (sequence, head, block of 64 tokens), keys and values apart:
+ *   k8, v8            [B, H, nblk, 4096] bytes (16-byte aligned); k_scale, v_scale [B, H, nblk]; lens [B]: tokens held
+ *   key of token t    bytes (t / 64) * 4096 + (t % 64) * 64 + dim
+ *   value of token t  byte  (t / 64) * 4096 + dim * 64 + p with t % 64 = ((p >> 2) & 3) * 16 + (p >> 4) * 4 + (p & 3)
+ * amax = largest magnitude of the block (at least 2^-100); T2S_KV_INT8: s = amax / 127; T2S_KV_E4M3: s = the least power of two with
+ * amax <= 448 s.  An element is held as the int8 / e4m3 number nearest to x r (r = 1 / s in fp32, exact product, ties to even) and stands for
+ * code * s.  A value that is not finite makes the scale of its block NaN.  A length outside 0 .. 64 nblk (an append that did not fit
+ * leaves -1) makes every result over its sequence NaN.
+ *
+ * t2s_kv8_append: token j of sequence b is row rows[b, j] (NULL: row j) of k / v, element (b, row, h, d) at batch_stride b + row_stride row +
+ *   head_stride h + d; counts[b] (NULL: T) of them are put behind lens[b], which is advanced.  0 <= row < L or the block turns NaN.  A block that
+ *   holds tokens already keeps the larger of its scale and the new tokens', and its old codes are rounded again where the scale grew.
+ *   ticket [B]: zeros on entry and on return (which workgroup ends last); one append on a cache at a time.
+ * t2s_kv8_dequantize: k, v [B, H, 64 nblk, 64] in dtype; zeros behind the length.
+ * t2s_kv8_attn: out[b, n, hq] = softmax(scale q . k) v over the lens[b] cached tokens of key head hq / G and then the first tail_len[b, n]
+ *   (NULL: tail_T) of the row's own tail_T tail tokens (tail_k / tail_v in dtype, element (b, n, t, h, d) by their strides; NULL: none);
+ *   lse: natural log-sum-exp [B, N, H G].  A row that sees nothing: out 0, lse -inf.  splits: shares of the token axis
+ *   (t2s_kv8_attn_splits for about max_tokens tokens; any positive number is right for any length); workspace as
+ *   t2s_kv8_attn_workspace_bytes says, contents on entry irrelevant. */
+#define T2S_KV_INT8 0
+#define T2S_KV_E4M3 1
+int t2s_kv8_append(const void* k, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                   int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride, const int32_t* rows, int64_t rows_batch_stride,
+                   const int32_t* counts, void* k8, void* v8, float* k_scale, float* v_scale, int32_t* lens, int32_t* ticket,
+                   int B, int H, int T, int L, int nblk, int dtype, int fmt, t2s_stream_t stream);
+int t2s_kv8_dequantize(const void* k8, const void* v8, const float* k_scale, const float* v_scale, const int32_t* lens, void* k, void* v,
+                       int B, int H, int nblk, int dtype, int fmt, t2s_stream_t stream);
+int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens);
+int64_t t2s_kv8_attn_workspace_bytes(int B, int N, int H, int G, int splits);
+int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride, const void* k8, const void* v8,
+                 const float* k_scale, const float* v_scale, const int32_t* lens, const void* tail_k, const void* tail_v,
+                 int64_t t_batch_stride, int64_t t_row_stride, int64_t t_token_stride, int64_t t_head_stride,
+                 const int32_t* tail_len, int64_t tl_batch_stride, int64_t tl_row_stride, int tail_T, void* out, float* lse,
+                 void* workspace, int64_t workspace_bytes, int splits, int B, int N, int H, int G, int nblk, float scale, int dtype,
+                 int fmt, t2s_stream_t stream);
+
+/* ---- answer decoding: beam search (vitxt_gqa_amd/csrc/beam.hip), the widened argmax of pythia/models/t2s.py:315-354 --------------------
+ * t2s_beam_select: of the N V candidates scores[b, n] + logits[b, n, v] - log sum exp(logits[b, n, :]) of each sequence the n_select
+ *   best, in descending order, ties to the lowest n V + v: out_scores [B, n_select] fp32, out_parents (n) and out_tokens (v) int64.
+ *   logits: element (b, n, v) at batch_stride b + beam_stride n + v, fp32 or bf16; NaN counts as -inf, +inf as the largest number.
+ *   finished [B, N] bytes or NULL: a beam that has ended offers `pad` at its own score and nothing else (its logits are not read).
+ *   Candidates at -inf are taken, lowest first, only when there are no others.  Scores are formed and compared in 64 bits.
+ *   N and n_select at most T2S_BEAM_MAX.  workspace: 8-byte aligned, t2s_beam_select_workspace_bytes, contents on entry irrelevant.
+ * t2s_beam_reorder: state is [outer, B, N] rows of row_bytes; the first used_bytes of row (o, b, n) become those of (o, b, parents[b, n]), in place.
+ *   A parent outside 0 .. N - 1 counts as the nearest. */
+#define T2S_BEAM_MAX 32
+int64_t t2s_beam_select_workspace_bytes(int B, int N, int V, int n_select);
+int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride, const float* scores, const uint8_t* finished, int pad,
+                    float* out_scores, int64_t* out_parents, int64_t* out_tokens, void* workspace, int64_t workspace_bytes,
+                    int B, int N, int V, int n_select, int dtype, t2s_stream_t stream);
+int t2s_beam_reorder(void* state, const int64_t* parents, int outer, int B, int N, int64_t row_bytes, int64_t used_bytes,
+                     t2s_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

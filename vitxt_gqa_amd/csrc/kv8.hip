@@ -1,0 +1,646 @@
+// The 8-bit key / value cache of answer decoding and the attention that reads it, for gfx950.
+//
+//  * t2s_kv8_append      quantises new K / V rows into the cache, behind each sequence's length, and advances the length
+//  * t2s_kv8_dequantize  what the cache holds, as [B, H, capacity, 64] rows in the operand dtype
+//  * t2s_kv8_attn        softmax(scale q K^T) V of a few query rows per sequence over [cache | the row's own tail]
+//
+// The decode step these serve is T2S._forward_mmt_and_output's eval loop (pythia/models/t2s.py:315-354): the prefix
+// [question; frames; OCR] of up to 10 120 rows is the same in every step and for every beam, the decoded tokens are few.
+//
+// Cache format.  Token t of a sequence lies in block t / 64; a block of one head is 4 096 bytes of keys and 4 096 of values with
+// one fp32 scale each.  amax = largest magnitude of the block's tokens (at least 2^-100); int8: s = amax / 127; e4m3: s = the
+// least power of two with amax <= 448 s.  An element x is the int8 / e4m3 number nearest to x r, r = 1 / s rounded to fp32, ties
+// to even, of the EXACT product (int8: one fma against 1.5 2^23; e4m3: a power-of-two product is exact): the code does not
+// depend on how the product is rounded.  A value that is not finite makes its block's scale NaN: visible, never a wrong number.
+//   keys    byte token * 64 + dim
+//   values  byte dim * 64 + p, position p = g * 16 + t * 4 + r holding token t * 16 + g * 4 + r
+// The value order is what the attention's registers hold: S^T = K Q^T by 16x16x32 MFMAs leaves lane (n = lane & 15, g = lane >> 4)
+// with the scores of query n against tokens t * 16 + g * 4 + r, and P^T is fed back as the B operand of O^T = V^T P^T without leaving the
+// lane; the 16 bytes a lane loads of value row `dim` are then the A operand against exactly those tokens.  No LDS, no
+// shuffles between the two products, and every load of the pass is 16 contiguous bytes per lane.
+#include "common.h"
+
+namespace {
+
+constexpr int KV_BLOCK = 64;                       // tokens per block
+constexpr int KV_HD = 64;                          // head dimension
+constexpr int KV_BYTES = KV_BLOCK * KV_HD;         // code bytes of a block (keys or values)
+constexpr float KV_LOG2E = 1.4426950408889634f;
+constexpr float KV_LN2 = 0.6931471805599453f;
+
+constexpr int FMT_INT8 = T2S_KV_INT8, FMT_E4M3 = T2S_KV_E4M3;
+
+__device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_u(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+// the block's scale from the bits of its largest magnitude (>= 0x7f800000: a value that is not finite -> NaN)
+template <int FMT>
+__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return as_f(0x7fc00000u);
+  const float a = fmaxf(as_f(amax_bits), 0x1p-100f);
+  if (FMT == FMT_INT8) return a / 127.0f;
+  const uint32_t u = as_u(a);                      // 448 = 1.75 * 2^8
+  return as_f(((u >> 23) - 8u + ((u & 0x7fffffu) > 0x600000u ? 1u : 0u)) << 23);
+}
+
+// four elements -> four codes; r = 1 / scale (0 for a block without a finite scale)
+template <int FMT>
+__device__ __forceinline__ uint32_t encode4(const float* x, float r) {
+  if (FMT == FMT_INT8) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (as_u(__builtin_fmaf(x[i], r, 12582912.0f)) & 0xffu) << (8 * i);      // nearest even of the exact product
+    return w;
+  }
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * r, x[1] * r, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * r, x[3] * r, w, true);
+}
+
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t w, float* x) {
+  if (FMT == FMT_INT8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+  } else {
+    typedef __attribute__((ext_vector_type(2))) float f2;
+    const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+  }
+}
+
+// eight codes -> the bf16 operand of an MFMA (exact: int8 and e4m3 fit bf16's eight significant bits)
+template <int FMT>
+__device__ __forceinline__ bf16x8 decode8(uint32_t lo, uint32_t hi) {
+  if (FMT == FMT_INT8) {
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (bf16_t)(float)(int8_t)(lo >> (8 * i));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[4 + i] = (bf16_t)(float)(int8_t)(hi >> (8 * i));
+    return r;
+  }
+  typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+  const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// word position of token group tg (tokens 4 tg .. 4 tg + 3) inside a value row: p / 4 of the order above
+__device__ __forceinline__ int v_word(int tg) { return (tg & 3) * 4 + (tg >> 2); }
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// append.  One workgroup = one (sequence, head, K or V) walking the blocks that the new tokens touch; a thread owns 4 tokens x 4 dims
+// of a block, so both storage orders are 32-bit words of it, and the words go out through a 4 KB LDS image as one contiguous block.
+struct AppendArgs {
+  const void* x[2];                                // K, V
+  int64_t x_bs[2], x_ts[2], x_hs[2];
+  const int32_t *rows, *counts;
+  int64_t rows_bs;
+  uint8_t *k8, *v8;
+  float *ks, *vs;
+  int32_t *lens, *ticket;
+  int B, H, T, L, nblk;
+};
+
+template <typename TX, int FMT>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
+  __shared__ __attribute__((aligned(16))) uint32_t img[KV_BYTES / 4];
+  __shared__ uint32_t red[4];
+  const int tid = threadIdx.x, tg = tid >> 4, dg = tid & 15;
+  const int which = blockIdx.y & 1, h = blockIdx.y >> 1, b = blockIdx.z;
+  const int len = a.lens[b];
+  const int cap = a.nblk * KV_BLOCK;
+  int n = a.counts ? a.counts[b] : a.T;
+  n = n < 0 ? 0 : (n > a.T ? a.T : n);
+  const bool poisoned = len < 0 || len > cap;
+  const int room = poisoned ? 0 : cap - len;
+  const bool over = n > room;
+  if (over) n = room;
+  if (!poisoned && n > 0) {
+    const TX* x = (const TX*)a.x[which] + (int64_t)b * a.x_bs[which] + (int64_t)h * a.x_hs[which] + dg * 4;
+    const int64_t x_ts = a.x_ts[which];
+    const int64_t base = ((int64_t)b * a.H + h) * a.nblk;
+    uint8_t* codes = which ? a.v8 : a.k8;
+    float* scales = which ? a.vs : a.ks;
+    const int first = len / KV_BLOCK, last = (len + n - 1) / KV_BLOCK;
+    for (int blk = first + blockIdx.x; blk <= last; blk += gridDim.x) {
+      uint8_t* dst = codes + (base + blk) * KV_BYTES;
+      const bool joins = blk == first && len % KV_BLOCK != 0;          // the block holds tokens already
+      const float s_old = joins ? scales[base + blk] : 0.f;
+      float val[4][4];                                                  // [token][dim]
+      uint32_t mx = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = blk * KV_BLOCK + tg * 4 + i - len;               // number of the new token
+        f32x4 f = {0.f, 0.f, 0.f, 0.f};
+        if (j >= 0 && j < n) {
+          int64_t row = a.rows ? a.rows[(int64_t)b * a.rows_bs + j] : j;
+          if (row >= 0 && row < a.L) f = Vec4<TX>::load(x + row * x_ts);
+          else f[0] = as_f(0x7fc00000u);                                // a row that is not there: the block turns NaN
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          val[i][d] = f[d];
+          mx = max(mx, as_u(f[d]) & 0x7fffffffu);
+        }
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
+      if ((tid & 63) == 0) red[tid >> 6] = mx;
+      if (joins) {                                                      // what the block holds, read before anyone writes (barrier below)
+        const uint32_t* src = (const uint32_t*)dst;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float old[4];
+          if (which == 0) {
+            decode4<FMT>(src[(tg * 4 + i) * 16 + dg], old);             // token tg * 4 + i, four dims
+            if (blk * KV_BLOCK + tg * 4 + i < len)
+#pragma unroll
+              for (int d = 0; d < 4; ++d) val[i][d] = old[d] * s_old;
+          } else {
+            decode4<FMT>(src[(dg * 4 + i) * 16 + v_word(tg)], old);     // dim dg * 4 + i, four tokens
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              if (blk * KV_BLOCK + tg * 4 + t < len) val[t][i] = old[t] * s_old;
+          }
+        }
+      }
+      __syncthreads();
+      mx = max(max(red[0], red[1]), max(red[2], red[3]));
+      float s = scale_of<FMT>(mx);
+      if (joins && !(s >= s_old)) s = s != s ? s : s_old;               // the larger of the two; a NaN on either side stays
+      const float r = s == s ? 1.0f / s : 0.f;
+      if (s != s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) val[i][d] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (which == 0) {
+          img[(tg * 4 + i) * 16 + dg] = encode4<FMT>(val[i], r);
+        } else {
+          const float col[4] = {val[0][i], val[1][i], val[2][i], val[3][i]};
+          img[(dg * 4 + i) * 16 + v_word(tg)] = encode4<FMT>(col, r);
+        }
+      }
+      __syncthreads();
+      ((uint4*)dst)[tid] = ((const uint4*)img)[tid];
+      if (tid == 0) scales[base + blk] = s;
+      // (the next round's barrier after `red` keeps its image writes behind this round's reads)
+    }
+  }
+  // the sequence's last workgroup advances its length: every other one has read it before it drew its ticket
+  __syncthreads();
+  if (tid == 0) {
+    const int total = (int)(gridDim.x * gridDim.y);
+    if (atomicAdd(a.ticket + b, 1) == total - 1) {
+      a.ticket[b] = 0;
+      a.lens[b] = poisoned || over ? -1 : len + n;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// read-back: one workgroup per (block walk, head and K / V, sequence)
+template <typename TX, int FMT>
+__global__ __launch_bounds__(256) void kv8_dequantize_kernel(const uint8_t* __restrict__ k8, const uint8_t* __restrict__ v8,
+                                                             const float* __restrict__ ks, const float* __restrict__ vs,
+                                                             const int32_t* __restrict__ lens, TX* __restrict__ k, TX* __restrict__ v,
+                                                             int H, int nblk) {
+  const int tid = threadIdx.x, tg = tid >> 4, dg = tid & 15;
+  const int which = blockIdx.y & 1, h = blockIdx.y >> 1, b = blockIdx.z;
+  const int len = lens[b];
+  const int64_t base = ((int64_t)b * H + h) * nblk;
+  const bool bad = len < 0 || len > nblk * KV_BLOCK;
+  const float none = bad ? as_f(0x7fc00000u) : 0.f;
+  for (int blk = blockIdx.x; blk < nblk; blk += gridDim.x) {
+    TX* out = (which ? v : k) + ((base + blk) * KV_BLOCK + tg * 4) * KV_HD + dg * 4;
+    float val[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) val[i][d] = none;
+    const int left = len - blk * KV_BLOCK - tg * 4;                     // tokens of this thread's four that are there
+    if (left > 0 && !bad) {
+      const uint32_t* src = (const uint32_t*)((which ? v8 : k8) + (base + blk) * KV_BYTES);
+      const float s = (which ? vs : ks)[base + blk];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float c[4];
+        if (which == 0) {
+          decode4<FMT>(src[(tg * 4 + i) * 16 + dg], c);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) val[i][d] = i < left ? c[d] * s : 0.f;
+        } else {
+          decode4<FMT>(src[(dg * 4 + i) * 16 + v_word(tg)], c);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) val[t][i] = t < left ? c[t] * s : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) Vec4<TX>::store(out + i * KV_HD, f32x4{val[i][0], val[i][1], val[i][2], val[i][3]});
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// attention.  R = N * G query rows (N rows of a sequence, G query heads per key head) share the keys of one (sequence, head).
+struct AttnArgs {
+  const void* q;
+  int64_t q_bs, q_ns, q_hs;
+  const uint8_t *k8, *v8;
+  const float *ks, *vs;
+  const int32_t* lens;
+  const void *tk, *tv;
+  int64_t t_bs, t_ns, t_ts, t_hs;
+  const int32_t* tail_len;
+  int64_t tl_bs, tl_ns;
+  int tail_T;
+  void* out;
+  float* lse;
+  float* part_o;        // [B * H][nsplit][R][64]
+  float* part_ml;       // [B * H][nsplit][R][2]: running maximum (log2 units), sum
+  float scale;
+  int B, N, H, G, nblk, nsplit, row_tiles;
+};
+
+// x as a sum of TERMS bf16 numbers (8 significant bits each): 1 for what is bf16 already, 2 keep 16 bits, 3 the whole of an fp32
+template <int TERMS>
+__device__ __forceinline__ void split_bf16(float x, bf16_t (&o)[TERMS]) {
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    o[i] = (bf16_t)x;
+    x -= (float)o[i];
+  }
+}
+
+// maximum / sum over the four 16-lane groups that hold one query's keys
+__device__ __forceinline__ float across_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ __forceinline__ float across_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+// One workgroup: one (sequence, head), one group of 16 QT query rows, one share of the blocks; its four waves take the blocks in turn,
+// each with its own running maximum / sum / O, and are joined through LDS at the end.
+template <typename TQ, int FMT, int QT>
+__global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
+  constexpr int TQN = sizeof(TQ) == 4 ? 3 : 1;     // bf16 terms of a query element
+  constexpr int TP = sizeof(TQ) == 4 ? 3 : 2;      // ... and of a probability
+  __shared__ __attribute__((aligned(16))) float o_s[4][16][KV_HD + 4];
+  __shared__ float m_s[4][16 * QT], l_s[4][16 * QT];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x % a.nsplit;
+  const int64_t rest = blockIdx.x / a.nsplit;
+  const int rt = (int)(rest % a.row_tiles);
+  const int64_t pair = rest / a.row_tiles;
+  const int b = (int)(pair / a.H), h = (int)(pair % a.H);
+  const int R = a.N * a.G, row0 = rt * 16 * QT;
+  const int len = a.lens[b];
+  const int blocks = len > 0 ? (min(len, a.nblk * KV_BLOCK) + KV_BLOCK - 1) / KV_BLOCK : 0;
+  const int b0 = (int)((int64_t)blocks * split / a.nsplit), b1 = (int)((int64_t)blocks * (split + 1) / a.nsplit);
+
+  // queries: B operand, lane (n, g) holds dims g * 16 + step * 8 .. + 7 of row n
+  bf16x8 qf[QT][2][TQN];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int row = row0 + t * 16 + n;
+    const int rc = row < R ? row : R - 1;
+    const TQ* qp = (const TQ*)a.q + (int64_t)b * a.q_bs + (int64_t)(rc / a.G) * a.q_ns + (int64_t)(h * a.G + rc % a.G) * a.q_hs + g * 16;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x4 f = Vec4<TQ>::load(qp + s * 8 + e * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          bf16_t w[TQN];
+          split_bf16<TQN>(f[i], w);
+#pragma unroll
+          for (int k = 0; k < TQN; ++k) qf[t][s][k][e * 4 + i] = w[k];
+        }
+      }
+  }
+  f32x4 o[QT][4];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float to_log2 = a.scale * KV_LOG2E;
+  const int64_t base = pair * a.nblk;
+  for (int blk = b0 + wave; blk < b1; blk += 4) {
+    const uint8_t* kp = a.k8 + (base + blk) * KV_BYTES + n * KV_HD + g * 16;
+    const uint8_t* vp = a.v8 + (base + blk) * KV_BYTES + n * KV_BLOCK + g * 16;
+    const float ks = a.ks[base + blk] * to_log2, vs = a.vs[base + blk];
+    uint4 kr[4], vr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kr[i] = *(const uint4*)(kp + i * 16 * KV_HD);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vr[i] = *(const uint4*)(vp + i * 16 * KV_BLOCK);
+    const int left = len - blk * KV_BLOCK;                  // tokens of the block that are there
+    if (left < KV_BLOCK) {                                  // codes behind the length count as zeros (an e4m3 NaN there would outlive p = 0)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t* w = (uint32_t*)&vr[i];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int k = left - (t * 16 + g * 4);
+          w[t] &= k >= 4 ? 0xffffffffu : (k <= 0 ? 0u : (1u << (8 * k)) - 1u);
+        }
+      }
+    }
+    bf16x8 kf[4][2], vf[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kf[i][0] = decode8<FMT>(kr[i].x, kr[i].y);
+      kf[i][1] = decode8<FMT>(kr[i].z, kr[i].w);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      vf[i][0] = decode8<FMT>(vr[i].x, vr[i].y);
+      vf[i][1] = decode8<FMT>(vr[i].z, vr[i].w);
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      float x[4][4];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int k = TQN - 1; k >= 0; --k) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][s], qf[t][s][k], acc, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[i][r] = i * 16 + g * 4 + r < left ? acc[r] * ks : -INFINITY;
+          mx = fmaxf(mx, x[i][r]);
+        }
+      }
+      mx = across_max(mx);
+      if (mx > m[t]) {
+        const float f = __builtin_amdgcn_exp2f(m[t] - mx);            // (0 the first time: exp2(-inf))
+        m[t] = mx;
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[t][d] *= f;
+      }
+      const float ms = m[t] == -INFINITY ? 0.f : m[t];
+      bf16x8 pf[2][TP];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(x[i][r] - ms);
+          l[t] += p;
+          bf16_t w[TP];
+          split_bf16<TP>(p * vs, w);
+#pragma unroll
+          for (int k = 0; k < TP; ++k) pf[i >> 1][k][(i & 1) * 4 + r] = w[k];
+        }
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int k = TP - 1; k >= 0; --k) o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d][s], pf[s][k], o[t][d], 0, 0, 0);
+    }
+  }
+  // ---- join the four waves
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const float ls = across_sum(l[t]);
+    if (g == 0) {
+      m_s[wave][t * 16 + n] = m[t];
+      l_s[wave][t * 16 + n] = ls;
+    }
+  }
+  for (int t = 0; t < QT; ++t) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) *(f32x4*)&o_s[wave][n][d * 16 + g * 4] = o[t][d];
+    __syncthreads();
+    const int r = tid >> 4, c = (tid & 15) * 4, row = row0 + t * 16 + r;
+    const float m0 = fmaxf(fmaxf(m_s[0][t * 16 + r], m_s[1][t * 16 + r]), fmaxf(m_s[2][t * 16 + r], m_s[3][t * 16 + r]));
+    const float ms = m0 == -INFINITY ? 0.f : m0;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    float ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(m_s[w][t * 16 + r] - ms);
+      sum += *(const f32x4*)&o_s[w][r][c] * f;
+      ls += l_s[w][t * 16 + r] * f;
+    }
+    if (row < R) {
+      const int64_t at = (pair * a.nsplit + split) * R + row;
+      *(f32x4*)(a.part_o + at * KV_HD + c) = sum;
+      if (c == 0) {
+        a.part_ml[at * 2] = m0;
+        a.part_ml[at * 2 + 1] = ls;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One wave per output row: joins the shares of the cache and the row's own tail (operand dtype, scored here in fp32).
+template <typename TQ>
+__global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
+  __shared__ float q_s[4][KV_HD];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int HQ = a.H * a.G, R = a.N * a.G;
+  const int64_t row = (int64_t)blockIdx.x * 4 + wave;           // b, n, query head
+  const int64_t rows = (int64_t)a.B * a.N * HQ;
+  const bool there = row < rows;
+  const int64_t rc = there ? row : rows - 1;
+  const int hq = (int)(rc % HQ), n = (int)(rc / HQ % a.N), b = (int)(rc / HQ / a.N);
+  const int h = hq / a.G, len = a.lens[b];
+  const int64_t at0 = ((int64_t)b * a.H + h) * a.nsplit * R + n * a.G + hq % a.G;
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const int64_t at = at0 + (int64_t)s * R;
+    const float ms = a.part_ml[at * 2], ls = a.part_ml[at * 2 + 1], os = a.part_o[at * KV_HD + lane];
+    const float mn = fmaxf(m, ms), mu = mn == -INFINITY ? 0.f : mn;
+    const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(ms - mu);
+    l = l * f0 + ls * f1;
+    o = o * f0 + os * f1;
+    m = mn;
+  }
+  const TQ* qp = (const TQ*)a.q + (int64_t)b * a.q_bs + (int64_t)n * a.q_ns + (int64_t)hq * a.q_hs;
+  q_s[wave][lane] = (float)qp[lane] * (a.scale * KV_LOG2E);
+  __syncthreads();
+  int T = 0;
+  if (a.tk) {
+    T = a.tail_len ? a.tail_len[(int64_t)b * a.tl_bs + (int64_t)n * a.tl_ns] : a.tail_T;
+    T = T < 0 ? 0 : (T > a.tail_T ? a.tail_T : T);
+  }
+  const TQ* tk = (const TQ*)a.tk + (int64_t)b * a.t_bs + (int64_t)n * a.t_ns + (int64_t)h * a.t_hs;
+  const TQ* tv = (const TQ*)a.tv + (int64_t)b * a.t_bs + (int64_t)n * a.t_ns + (int64_t)h * a.t_hs;
+  for (int t0 = 0; t0 < T; t0 += 64) {
+    float x = -INFINITY;
+    if (t0 + lane < T) {
+      x = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < KV_HD; d += 4) {
+        const f32x4 kv = Vec4<TQ>::load(tk + (int64_t)(t0 + lane) * a.t_ts + d);
+        x += kv[0] * q_s[wave][d] + kv[1] * q_s[wave][d + 1] + kv[2] * q_s[wave][d + 2] + kv[3] * q_s[wave][d + 3];
+      }
+    }
+    float mx = x;
+#pragma unroll
+    for (int i = 32; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i, 64));
+    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
+    const float f0 = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(x - mu);
+    l = l * f0 + wave_sum(p);
+    o *= f0;
+    m = mn;
+    const int nt = min(64, T - t0);
+    for (int t = 0; t < nt; ++t) o += __shfl(p, t, 64) * (float)tv[(int64_t)(t0 + t) * a.t_ts + lane];
+  }
+  if (there) {
+    // a row that sees nothing: zeros, lse = -inf; a sequence whose length is none (it overflowed on the device): NaN
+    const bool bad = len < 0 || len > a.nblk * KV_BLOCK;
+    const float nan = as_f(0x7fc00000u);
+    const float res = bad ? nan : (l == 0.f ? 0.f : o / l);
+    ((TQ*)a.out)[row * KV_HD + lane] = (TQ)res;
+    if (lane == 0) a.lse[row] = bad ? nan : (l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * KV_LN2);
+  }
+}
+
+template <typename TQ, int FMT>
+void launch_attn(const AttnArgs& a, int qt, unsigned grid, hipStream_t st) {
+  if (qt == 1) hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 1>), dim3(grid), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 2>), dim3(grid), dim3(256), 0, st, a);
+}
+
+bool kv8_bad_fmt(int fmt) { return fmt != FMT_INT8 && fmt != FMT_E4M3; }
+
+// query tiles (of 16 rows) per workgroup
+int attn_row_tiles(int rows) { return rows > 16 ? 2 : 1; }
+
+}  // namespace
+
+extern "C" int t2s_kv8_append(const void* k, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                              int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride, const int32_t* rows, int64_t rows_batch_stride, const int32_t* counts, void* k8, void* v8, float* k_scale,
+                              float* v_scale, int32_t* lens, int32_t* ticket, int B, int H, int T, int L, int nblk, int dtype, int fmt,
+                              t2s_stream_t stream) {
+  T2S_CHECK_ARG(k && v && k8 && v8 && k_scale && v_scale && lens && ticket, "kv8_append: null pointer");
+  T2S_CHECK_ARG(B > 0 && B <= 65535 && H > 0 && H <= 32767 && T > 0 && L > 0 && nblk > 0 && nblk < (1 << 25), "kv8_append: bad shape B=%d H=%d T=%d L=%d nblk=%d", B, H, T, L, nblk);
+  T2S_CHECK_ARG(rows || T <= L, "kv8_append: %d tokens of %d rows", T, L);
+  T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "kv8_append: bad dtype %d", dtype);
+  T2S_CHECK_ARG(!kv8_bad_fmt(fmt), "kv8_append: bad format %d", fmt);
+  const int al = dtype == T2S_F32 ? 16 : 8;
+  T2S_CHECK_ARG((uintptr_t)k % al == 0 && (uintptr_t)v % al == 0 && k_batch_stride % 4 == 0 && k_row_stride % 4 == 0 && k_head_stride % 4 == 0 &&
+                    v_batch_stride % 4 == 0 && v_row_stride % 4 == 0 && v_head_stride % 4 == 0,
+                "kv8_append: rows must be aligned to 4 elements");
+  T2S_CHECK_ARG((uintptr_t)k8 % 16 == 0 && (uintptr_t)v8 % 16 == 0, "kv8_append: the cache must be aligned to 16 bytes");
+  AppendArgs a{{k, v}, {k_batch_stride, v_batch_stride}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride}, rows, counts, rows_batch_stride, (uint8_t*)k8, (uint8_t*)v8,
+               k_scale, v_scale, lens, ticket, B, H, T, L, nblk};
+  const int touched = (int)((T + 62LL) / 64 + 1);
+  // enough workgroups to fill the card (8 of them run on a CU), no more: each draws a ticket of its sequence when it ends
+  const int64_t pairs = (int64_t)B * H * 2;
+  int64_t gx = (8192 + pairs - 1) / pairs;
+  if (gx > touched) gx = touched;
+  dim3 grid((unsigned)gx, (unsigned)(2 * H), (unsigned)B), block(256);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == T2S_BF16 && fmt == FMT_INT8) hipLaunchKernelGGL((kv8_append_kernel<bf16_t, FMT_INT8>), grid, block, 0, st, a);
+  else if (dtype == T2S_BF16) hipLaunchKernelGGL((kv8_append_kernel<bf16_t, FMT_E4M3>), grid, block, 0, st, a);
+  else if (fmt == FMT_INT8) hipLaunchKernelGGL((kv8_append_kernel<float, FMT_INT8>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((kv8_append_kernel<float, FMT_E4M3>), grid, block, 0, st, a);
+  T2S_CHECK_LAUNCH("kv8_append");
+  return 0;
+}
+
+extern "C" int t2s_kv8_dequantize(const void* k8, const void* v8, const float* k_scale, const float* v_scale, const int32_t* lens, void* k,
+                                  void* v, int B, int H, int nblk, int dtype, int fmt, t2s_stream_t stream) {
+  T2S_CHECK_ARG(k8 && v8 && k_scale && v_scale && lens && k && v, "kv8_dequantize: null pointer");
+  T2S_CHECK_ARG(B > 0 && B <= 65535 && H > 0 && H <= 32767 && nblk > 0 && nblk < (1 << 25), "kv8_dequantize: bad shape B=%d H=%d nblk=%d", B, H, nblk);
+  T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "kv8_dequantize: bad dtype %d", dtype);
+  T2S_CHECK_ARG(!kv8_bad_fmt(fmt), "kv8_dequantize: bad format %d", fmt);
+  T2S_CHECK_ARG((uintptr_t)k8 % 16 == 0 && (uintptr_t)v8 % 16 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, "kv8_dequantize: 16-byte alignment");
+  const int64_t pairs = (int64_t)B * H * 2;
+  int64_t gx = (16384 + pairs - 1) / pairs;
+  if (gx > nblk) gx = nblk;
+  dim3 grid((unsigned)gx, (unsigned)(2 * H), (unsigned)B), block(256);
+  hipStream_t st = (hipStream_t)stream;
+  const uint8_t *a = (const uint8_t*)k8, *c = (const uint8_t*)v8;
+  if (dtype == T2S_BF16 && fmt == FMT_INT8)
+    hipLaunchKernelGGL((kv8_dequantize_kernel<bf16_t, FMT_INT8>), grid, block, 0, st, a, c, k_scale, v_scale, lens, (bf16_t*)k, (bf16_t*)v, H, nblk);
+  else if (dtype == T2S_BF16)
+    hipLaunchKernelGGL((kv8_dequantize_kernel<bf16_t, FMT_E4M3>), grid, block, 0, st, a, c, k_scale, v_scale, lens, (bf16_t*)k, (bf16_t*)v, H, nblk);
+  else if (fmt == FMT_INT8)
+    hipLaunchKernelGGL((kv8_dequantize_kernel<float, FMT_INT8>), grid, block, 0, st, a, c, k_scale, v_scale, lens, (float*)k, (float*)v, H, nblk);
+  else
+    hipLaunchKernelGGL((kv8_dequantize_kernel<float, FMT_E4M3>), grid, block, 0, st, a, c, k_scale, v_scale, lens, (float*)k, (float*)v, H, nblk);
+  T2S_CHECK_LAUNCH("kv8_dequantize");
+  return 0;
+}
+
+extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens) {
+  if (B <= 0 || N <= 0 || H <= 0 || G <= 0) return 0;
+  const int blocks = max_tokens > 0 ? (max_tokens + KV_BLOCK - 1) / KV_BLOCK : 1;
+  const int rows = N * G, qt = attn_row_tiles(rows);
+  const int64_t pairs = (int64_t)B * H * ((rows + 16 * qt - 1) / (16 * qt));
+  int64_t s = (2048 + pairs - 1) / pairs;
+  const int64_t most = (blocks + 7) / 8;          // two blocks at least for each wave of a share
+  if (s > most) s = most;
+  return (int)(s < 1 ? 1 : s);
+}
+
+extern "C" int64_t t2s_kv8_attn_workspace_bytes(int B, int N, int H, int G, int splits) {
+  return (int64_t)B * H * splits * N * G * (KV_HD + 2) * 4;
+}
+
+extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride, const void* k8, const void* v8,
+                            const float* k_scale, const float* v_scale, const int32_t* lens, const void* tail_k, const void* tail_v,
+                            int64_t t_batch_stride, int64_t t_row_stride, int64_t t_token_stride, int64_t t_head_stride,
+                            const int32_t* tail_len, int64_t tl_batch_stride, int64_t tl_row_stride, int tail_T, void* out, float* lse,
+                            void* workspace, int64_t workspace_bytes, int splits, int B, int N, int H, int G, int nblk, float scale, int dtype,
+                            int fmt, t2s_stream_t stream) {
+  T2S_CHECK_ARG(q && k8 && v8 && k_scale && v_scale && lens && out && lse && workspace, "kv8_attn: null pointer");
+  T2S_CHECK_ARG(B > 0 && N > 0 && H > 0 && G > 0 && nblk > 0 && nblk < (1 << 25) && (int64_t)N * G < (1 << 24) && (int64_t)B * H < (1 << 24),
+                "kv8_attn: bad shape B=%d N=%d H=%d G=%d nblk=%d", B, N, H, G, nblk);
+  T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "kv8_attn: bad dtype %d", dtype);
+  T2S_CHECK_ARG(!kv8_bad_fmt(fmt), "kv8_attn: bad format %d", fmt);
+  T2S_CHECK_ARG((tail_k == nullptr) == (tail_v == nullptr) && tail_T >= 0, "kv8_attn: tail keys and values come together");
+  const int al = dtype == T2S_F32 ? 16 : 8;
+  T2S_CHECK_ARG((uintptr_t)q % al == 0 && q_batch_stride % 4 == 0 && q_row_stride % 4 == 0 && q_head_stride % 4 == 0, "kv8_attn: query rows must be aligned to 4 elements");
+  T2S_CHECK_ARG((uintptr_t)tail_k % al == 0 && (uintptr_t)tail_v % al == 0 && t_batch_stride % 4 == 0 && t_row_stride % 4 == 0 && t_token_stride % 4 == 0 &&
+                    t_head_stride % 4 == 0, "kv8_attn: tail rows must be aligned to 4 elements");
+  T2S_CHECK_ARG((uintptr_t)k8 % 16 == 0 && (uintptr_t)v8 % 16 == 0 && (uintptr_t)workspace % 16 == 0, "kv8_attn: cache and workspace must be aligned to 16 bytes");
+  T2S_CHECK_ARG(splits >= 1 && workspace_bytes >= t2s_kv8_attn_workspace_bytes(B, N, H, G, splits), "kv8_attn: workspace of %lld bytes is too small for %d shares",
+                (long long)workspace_bytes, splits);
+  const int rows = N * G, qt = attn_row_tiles(rows);
+  AttnArgs a;
+  a.q = q; a.q_bs = q_batch_stride; a.q_ns = q_row_stride; a.q_hs = q_head_stride;
+  a.k8 = (const uint8_t*)k8; a.v8 = (const uint8_t*)v8; a.ks = k_scale; a.vs = v_scale; a.lens = lens;
+  a.tk = tail_T > 0 ? tail_k : nullptr; a.tv = tail_v; a.t_bs = t_batch_stride; a.t_ns = t_row_stride; a.t_ts = t_token_stride; a.t_hs = t_head_stride;
+  a.tail_len = tail_len; a.tl_bs = tl_batch_stride; a.tl_ns = tl_row_stride; a.tail_T = tail_T;
+  a.out = out; a.lse = lse;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o + (int64_t)B * H * splits * rows * KV_HD;
+  a.scale = scale; a.B = B; a.N = N; a.H = H; a.G = G; a.nblk = nblk; a.nsplit = splits; a.row_tiles = (rows + 16 * qt - 1) / (16 * qt);
+  const int64_t grid = (int64_t)B * H * a.row_tiles * splits, join = ((int64_t)B * N * H * G + 3) / 4;
+  T2S_CHECK_ARG(grid < ((int64_t)1 << 31) && join < ((int64_t)1 << 31), "kv8_attn: too many workgroups");
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == T2S_BF16) {
+    if (fmt == FMT_INT8) launch_attn<bf16_t, FMT_INT8>(a, qt, (unsigned)grid, st);
+    else launch_attn<bf16_t, FMT_E4M3>(a, qt, (unsigned)grid, st);
+    T2S_CHECK_LAUNCH("kv8_attn");
+    hipLaunchKernelGGL(kv8_attn_join_kernel<bf16_t>, dim3((unsigned)join), dim3(256), 0, st, a);
+  } else {
+    if (fmt == FMT_INT8) launch_attn<float, FMT_INT8>(a, qt, (unsigned)grid, st);
+    else launch_attn<float, FMT_E4M3>(a, qt, (unsigned)grid, st);
+    T2S_CHECK_LAUNCH("kv8_attn");
+    hipLaunchKernelGGL(kv8_attn_join_kernel<float>, dim3((unsigned)join), dim3(256), 0, st, a);
+  }
+  T2S_CHECK_LAUNCH("kv8_attn_join");
+  return 0;
+}

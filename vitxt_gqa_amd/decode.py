@@ -1,0 +1,267 @@
+"""Operators of answer decoding: an 8-bit key / value cache, the attention that reads it, and beam search's two steps.
+
+The eval loop of ``T2S`` (pythia/models/t2s.py:315-354) decodes 12 tokens against one long prefix [question; frames; OCR].  ``T2S.set_decoding``
+runs it on these operators (t2s.py ``_beam_decode``); they are also usable on their own:
+
+    cache = KVCache8(batch, heads, capacity, fmt="int8")                 # one layer
+    cache.append(k, v, counts=keys.cnt, rows=keys.idx)                   # the visible rows of the prefix
+    out, lse = attend(q, cache, tail_k, tail_v, tail_len)                # a few query rows, each with its own decoded tokens in the tail
+    scores, parents, tokens = beam_select(logits, scores, n_beams, finished, pad)
+    beam_reorder(tail, parents, batch_dim=1)
+
+Thin wrappers over the C ABI (``include/t2s_hip.h``; kernels in ``csrc/kv8.hip`` and ``csrc/beam.hip``): shapes, types, strides and devices are
+checked on the host, everything runs on the current stream of the tensors' device, without a synchronisation and without state other than
+the cache's own tensors - a step may be captured into a graph.  No gradients: the operands may not require any."""
+import contextlib
+
+import torch
+
+from . import hipext as X
+
+BLOCK = 64                  # tokens of a block: one scale for its keys and one for its values per head
+HEAD_DIM = 64
+BEAM_MAX = X.T2S_BEAM_MAX   # beams, and candidates a selection returns
+FORMATS = {"int8": (X.T2S_KV_INT8, torch.int8), "e4m3": (X.T2S_KV_E4M3, torch.float8_e4m3fn)}
+_NULL = contextlib.nullcontext()
+
+
+def _need(ok, msg, *args):
+    if not ok:
+        raise ValueError(msg % args if args else msg)
+
+
+def _on(device, *tensors):
+    """All of ``tensors`` (None: absent) on ``device``, a GPU; returns the context in which its current stream is the one to launch on."""
+    if device.type != "cuda":
+        raise RuntimeError("T2S HIP kernels need device tensors (got a %s tensor); there is no CPU path" % device)
+    for t in tensors:
+        if t is not None:
+            _need(t.device == device, "tensors on %s and %s: all of a call's tensors live on one device", device, t.device)
+            _need(not (t.requires_grad and torch.is_grad_enabled()), "the decode operators have no gradients: call them under torch.no_grad() or on detached tensors")
+    return _NULL if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _head_rows(t, name):
+    """[..., heads, 64] with dense 64-element rows that start at multiples of 4 elements."""
+    _need(t.dtype in (torch.bfloat16, torch.float32), "%s: float32 or bfloat16, got %s", name, t.dtype)
+    _need(t.shape[-1] == HEAD_DIM, "%s: the kernels are built for head_dim 64, got %s", name, tuple(t.shape))
+    ok = t.stride(-1) == 1 and t.data_ptr() % (4 * t.element_size()) == 0 and not any(s % 4 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+    _need(ok, "%s: rows of 64 dense elements, aligned to 4 elements, are needed (strides %s): call .contiguous()", name, t.stride())
+
+
+class KVCache8:
+    """Keys and values of ``batch`` sequences, ``heads`` heads of 64 dims and up to ``capacity`` tokens (rounded up to blocks of 64) in 8 bits.
+
+    ``fmt``: "int8" (an even grid of 127 steps up to the block's largest magnitude: the finer one for projections without outliers) or "e4m3"
+    (floating point, 3 fraction bits: keeps small values next to large ones).  One fp32 scale for each block of 64 tokens and head, keys and
+    values apart; the storage layout is part of the C ABI (``t2s_kv8_append`` in include/t2s_hip.h).  ``k``, ``v`` [B, H, blocks, 64, 64]
+    codes, ``k_scale``, ``v_scale`` [B, H, blocks], ``lens`` [B] int32: the tokens each sequence holds.
+
+    The cache is one object of the stream's order: two appends at a time, or an append while another stream reads, are the caller's race."""
+
+    def __init__(self, batch, heads, capacity, fmt="int8", device="cuda"):
+        _need(fmt in FORMATS, "KVCache8: unknown format %r (int8 or e4m3)", fmt)
+        _need(batch > 0 and heads > 0 and capacity > 0, "KVCache8: bad shape batch=%d heads=%d capacity=%d", batch, heads, capacity)
+        n = -(-int(capacity) // BLOCK)
+        dev = torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        code = FORMATS[fmt][1]
+        # (codes are written whole blocks at a time and read only below a sequence's length: nothing has to be cleared)
+        k, v = (torch.empty(batch, heads, n, BLOCK, HEAD_DIM, dtype=torch.uint8, device=dev).view(code) for _ in range(2))
+        ks, vs = (torch.zeros(batch, heads, n, dtype=torch.float32, device=dev) for _ in range(2))
+        self._adopt(k, v, ks, vs, torch.zeros(batch, dtype=torch.int32, device=dev), 0)
+
+    @classmethod
+    def from_parts(cls, k, v, k_scale, v_scale, lens, max_len=None):
+        """A cache around existing storage (used as it is, not copied): codes int8 or float8_e4m3fn [B, H, blocks, 64, 64], scales, lens.
+        ``max_len``: a bound on the lengths, if known; it only shapes the attention's launch."""
+        self = cls.__new__(cls)
+        self._adopt(k, v, k_scale, v_scale, lens, max_len)
+        return self
+
+    def _adopt(self, k, v, ks, vs, lens, max_len):
+        fmt = [f for f, (_, t) in FORMATS.items() if t == k.dtype]
+        _need(fmt and v.dtype == k.dtype, "KVCache8: codes are int8 or float8_e4m3fn, got %s and %s", k.dtype, v.dtype)
+        _need(k.dim() == 5 and k.shape[3:] == (BLOCK, HEAD_DIM) and v.shape == k.shape and k.numel() > 0, "KVCache8: codes [B, H, blocks, 64, 64], got %s and %s", tuple(k.shape), tuple(v.shape))
+        B, H, n = k.shape[:3]
+        _need(ks.shape == (B, H, n) and vs.shape == (B, H, n) and ks.dtype == vs.dtype == torch.float32, "KVCache8: scales are float32 [B, H, blocks]")
+        _need(lens.shape == (B,) and lens.dtype == torch.int32, "KVCache8: lens is int32 [B]")
+        for t in (k, v, ks, vs, lens):
+            _need(t.is_contiguous(), "KVCache8: the storage has to be contiguous")
+            _need(t.device == k.device, "KVCache8: the storage has to live on one device")
+        self.fmt, self._fmt = fmt[0], FORMATS[fmt[0]][0]
+        self.k, self.v, self.k_scale, self.v_scale, self.lens = k, v, ks, vs, lens
+        self.batch, self.heads, self.blocks, self.capacity, self.device = B, H, n, n * BLOCK, k.device
+        self.max_len = self.capacity if max_len is None else min(int(max_len), self.capacity)
+        self._ticket = torch.zeros(B, dtype=torch.int32, device=k.device)
+
+    def append(self, k, v, counts=None, rows=None):
+        """Puts new tokens behind what each sequence holds.  k, v: [B, R, H, 64] float32 or bfloat16, dense 64-element rows (slices of a fused
+        projection are fine).  ``rows`` int32 [B, T]: token j of sequence b is row rows[b, j] of them (T = R and row j without it; an
+        ``ops.KeyList``'s ``idx`` fits); ``counts`` int32 [B]: how many of the T tokens are appended (all, without it; more than T counts as T,
+        less than 0 as 0).  Returns self.
+
+        A block that holds tokens already keeps the larger of its scale and the new tokens' one; its codes are rounded again where it grew.
+        A value that is not finite, or a row number outside 0 .. R - 1, turns its block of that head to NaN.  Tokens that do not fit turn the
+        sequence's length to -1 and every result over it to NaN, until ``set_lens`` (the lengths live on the device: nothing is waited for)."""
+        _need(k.dim() == 4 and k.shape[0] == self.batch and k.shape[2] == self.heads and v.shape == k.shape and v.dtype == k.dtype,
+              "append: k and v [%d, R, %d, 64] of one type, got %s %s and %s %s", self.batch, self.heads, tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
+        R = k.shape[1]
+        T = R
+        if rows is not None:
+            _need(rows.dim() == 2 and rows.shape[0] == self.batch and rows.dtype == torch.int32 and (rows.shape[1] < 2 or rows.stride(1) == 1),
+                  "append: rows is int32 [%d, T] with dense rows, got %s %s", self.batch, tuple(rows.shape), rows.dtype)
+            T = rows.shape[1]
+        if counts is not None:
+            _need(counts.shape == (self.batch,) and counts.dtype == torch.int32 and counts.is_contiguous(), "append: counts is a dense int32 [%d]", self.batch)
+        _need(counts is not None or T <= self.capacity, "append: %d tokens do not fit a capacity of %d", T, self.capacity)
+        _need(R > 0 or T == 0, "append: %d tokens of no rows", T)
+        if T:
+            _head_rows(k, "append: k")
+            _head_rows(v, "append: v")
+        with _on(self.device, k, v, counts, rows):
+            if T == 0:
+                return self
+            X.check(X.lib().t2s_kv8_append(k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], None if rows is None else rows.data_ptr(),
+                                           0 if rows is None else rows.stride(0), None if counts is None else counts.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
+                                           self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.lens.data_ptr(), self._ticket.data_ptr(),
+                                           self.batch, self.heads, T, R, self.blocks, X.dtype_code(k), self._fmt, X.stream()), "t2s_kv8_append")
+        self.max_len = min(self.capacity, self.max_len + T)
+        return self
+
+    def set_lens(self, lens, max_len=None):
+        """Sets how many tokens each sequence holds: an int for all, or int32 [B] on the device.  Takes tokens back (a prefix is kept for another
+        continuation; 0 empties the cache); it cannot bring any in, and never more may be named than have been appended.  ``max_len`` as in
+        ``from_parts``."""
+        if isinstance(lens, int):
+            _need(0 <= lens <= self.capacity, "set_lens: %d outside 0 .. %d", lens, self.capacity)
+            self.lens.fill_(lens)
+            self.max_len = lens
+        else:
+            _need(lens.shape == (self.batch,) and lens.dtype == torch.int32, "set_lens: an int or int32 [%d], got %s %s", self.batch, tuple(lens.shape), lens.dtype)
+            self.lens.copy_(lens)
+        if max_len is not None:
+            self.max_len = max(0, min(int(max_len), self.capacity))
+        return self
+
+    def dequantize(self, dtype=torch.bfloat16):
+        """(keys, values) [B, H, capacity, 64] in ``dtype`` (float32 or bfloat16): code * scale, zeros behind a sequence's length."""
+        _need(dtype in (torch.bfloat16, torch.float32), "dequantize: float32 or bfloat16, got %s", dtype)
+        with _on(self.device):
+            k, v = (torch.empty(self.batch, self.heads, self.capacity, HEAD_DIM, dtype=dtype, device=self.device) for _ in range(2))
+            X.check(X.lib().t2s_kv8_dequantize(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.lens.data_ptr(),
+                                               k.data_ptr(), v.data_ptr(), self.batch, self.heads, self.blocks, X.dtype_code(k), self._fmt, X.stream()), "t2s_kv8_dequantize")
+        return k, v
+
+
+def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
+    """softmax(scale q k^T) v of a few query rows per sequence over what ``cache`` holds, then over each row's own tail.
+
+    q: [B, N, HQ, 64] float32 or bfloat16 (dense 64-element rows); HQ a multiple of the cache's heads: query head i reads key head
+    i // (HQ / heads).  tail_k, tail_v: [B, N, T, heads, 64] in q's type, the same strides (0 strides are fine: rows of one sequence may share
+    a tail), tokens that are in no cache - a beam's decoded steps, up to a few hundred; ``tail_len``: how many of the T each row sees, int or int32
+    [B, N] (all, without it; below 0 counts as 0, above T as T).  Returns (out [B, N, HQ, 64] in q's type, lse [B, N, HQ] float32: the natural
+    log-sum-exp of the scaled scores).  A row that sees no token at all: out 0, lse -inf.
+
+    Codes enter the matrix pipe as exact bf16; a query in float32 as the three bf16 terms that make it up; probabilities as two terms (bfloat16
+    results: 16 bits, below the rounding of the result) or three (float32).  All sums, maxima and scales are float32; the result is rounded once."""
+    _need(q.dim() == 4 and q.shape[0] == cache.batch and q.shape[2] > 0 and q.shape[2] % cache.heads == 0,
+          "attend: q [%d, N, a multiple of %d, 64], got %s", cache.batch, cache.heads, tuple(q.shape))
+    B, N, HQ, _ = q.shape
+    T, tk, tv, ts, tl, tls = 0, None, None, (0, 0, 0, 0), None, (0, 0)
+    _need((tail_k is None) == (tail_v is None), "attend: tail_k and tail_v come together")
+    _head_rows(q, "attend: q")
+    if tail_k is not None:
+        T = tail_k.shape[2] if tail_k.dim() == 5 else -1
+        _need(tuple(tail_k.shape) == (B, N, T, cache.heads, HEAD_DIM) and tail_v.shape == tail_k.shape and tail_k.dtype == q.dtype and tail_v.dtype == q.dtype,
+              "attend: tails [%d, %d, T, %d, 64] of q's type, got %s %s and %s %s", B, N, cache.heads, tuple(tail_k.shape), tail_k.dtype, tuple(tail_v.shape), tail_v.dtype)
+        if torch.is_tensor(tail_len):
+            _need(tail_len.shape == (B, N) and tail_len.dtype == torch.int32, "attend: tail_len is an int or int32 [%d, %d]", B, N)
+            tl, tls = tail_len, tail_len.stride()
+        elif tail_len is not None:
+            T = max(0, min(int(tail_len), T))
+        if T > 0:
+            _head_rows(tail_k, "attend: tail_k")
+            _head_rows(tail_v, "attend: tail_v")
+            _need(tail_k.stride() == tail_v.stride(), "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
+            tk, tv, ts = tail_k.data_ptr(), tail_v.data_ptr(), tail_k.stride()[:4]
+    else:
+        _need(tail_len is None, "attend: tail_len without a tail")
+    with _on(cache.device, q, tail_k, tail_v, tl):
+        out = torch.empty(B, N, HQ, HEAD_DIM, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, N, HQ, dtype=torch.float32, device=q.device)
+        if N == 0:
+            return out, lse
+        G = HQ // cache.heads
+        lib = X.lib()
+        splits = lib.t2s_kv8_attn_splits(B, N, cache.heads, G, cache.max_len)
+        nbytes = lib.t2s_kv8_attn_workspace_bytes(B, N, cache.heads, G, splits)
+        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+        X.check(lib.t2s_kv8_attn(q.data_ptr(), *q.stride()[:3], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+                                 cache.lens.data_ptr(), tk, tv, *ts, None if tl is None else tl.data_ptr(), *tls, T, out.data_ptr(), lse.data_ptr(),
+                                 ws.data_ptr(), nbytes, splits, B, N, cache.heads, G, cache.blocks, float(scale), X.dtype_code(q), cache._fmt, X.stream()), "t2s_kv8_attn")
+    return out, lse
+
+
+def beam_select(logits, scores, n_select, finished=None, pad=0):
+    """The ``n_select`` best continuations of each sequence's beams.
+
+    logits [B, N, V] float32 or bfloat16 (dense rows), scores [B, N] float32: the beams' summed log-probabilities (-inf: no beam; the first step
+    starts from one beam at 0 and the others at -inf).  A candidate (n, v) scores scores[b, n] + logits[b, n, v] - logsumexp(logits[b, n]).
+    ``finished`` bool [B, N]: a beam that has ended offers the token ``pad`` at its own score and nothing else.  NaN logits count as -inf, +inf as
+    the largest number.  Returns (scores [B, n_select] float32, parents int64: the beam n, tokens int64: the word v), best first, ties to the lowest
+    n V + v; candidates at -inf only where nothing else is left.  At most 32 beams and 32 candidates."""
+    _need(logits.dim() == 3 and logits.shape[2] > 0 and logits.shape[1] > 0, "beam_select: logits [B, N, V], got %s", tuple(logits.shape))
+    B, N, V = logits.shape
+    K = int(n_select)
+    _need(logits.dtype in (torch.bfloat16, torch.float32), "beam_select: float32 or bfloat16 logits, got %s", logits.dtype)
+    _need(V == 1 or logits.stride(2) == 1, "beam_select: dense rows of logits are needed (strides %s): call .contiguous()", logits.stride())
+    _need(scores.shape == (B, N) and scores.dtype == torch.float32, "beam_select: scores is float32 [%d, %d], got %s %s", B, N, tuple(scores.shape), scores.dtype)
+    _need(N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V, "beam_select: %d of %d x %d candidates (at most %d beams and %d candidates)", K, N, V, BEAM_MAX, BEAM_MAX)
+    _need(0 <= pad < V, "beam_select: pad %d outside the vocabulary of %d", pad, V)
+    if finished is not None:
+        _need(finished.shape == (B, N) and finished.dtype in (torch.bool, torch.uint8), "beam_select: finished is bool [%d, %d], got %s %s", B, N, tuple(finished.shape), finished.dtype)
+    with _on(logits.device, logits, scores, finished):
+        out = torch.empty(B, K, dtype=torch.float32, device=logits.device)
+        parents, tokens = torch.empty(2, B, K, dtype=torch.int64, device=logits.device).unbind(0)
+        if B == 0:
+            return out, parents, tokens
+        scores = scores.contiguous()
+        if finished is not None:
+            finished = finished.contiguous()
+        lib = X.lib()
+        nbytes = lib.t2s_beam_select_workspace_bytes(B, N, V, K)
+        ws = torch.empty((nbytes + 7) // 8, dtype=torch.int64, device=logits.device)
+        X.check(lib.t2s_beam_select(logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), None if finished is None else finished.data_ptr(), int(pad),
+                                    out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, X.dtype_code(logits), X.stream()), "t2s_beam_select")
+    return out, parents, tokens
+
+
+def beam_reorder(state, parents, batch_dim=0, used=None):
+    """state[.., b, n, ..] = state[.., b, parents[b, n], ..] in place, for every beam at once; returns ``state``.
+
+    state: contiguous, any type; its axes ``batch_dim`` and ``batch_dim + 1`` are the sequences and their beams.  parents int64 [B, N]: any beam any
+    number of times (outside 0 .. N - 1 counts as the nearest).  ``used``: only the first ``used`` entries of the axis behind the beams are moved
+    (the steps decoded so far); the rest is left as it is.  At most 32 beams."""
+    d = batch_dim + state.dim() if batch_dim < 0 else batch_dim
+    _need(0 <= d and d + 2 <= state.dim(), "beam_reorder: batch_dim %d of a %d-d state", batch_dim, state.dim())
+    B, N = state.shape[d], state.shape[d + 1]
+    _need(state.is_contiguous(), "beam_reorder: the state has to be contiguous (strides %s)", state.stride())
+    _need(N <= BEAM_MAX, "beam_reorder: at most %d beams, got %d", BEAM_MAX, N)
+    _need(parents.shape == (B, N) and parents.dtype == torch.int64, "beam_reorder: parents is int64 [%d, %d], got %s %s", B, N, tuple(parents.shape), parents.dtype)
+    rest = state.shape[d + 2:]
+    row = state.element_size()
+    for s in rest:
+        row *= s
+    nbytes = row
+    if used is not None:
+        _need(len(rest) > 0 and 0 <= used <= rest[0], "beam_reorder: used %s of %s", used, tuple(rest))
+        nbytes = row // max(1, rest[0]) * int(used)
+    outer = 1
+    for s in state.shape[:d]:
+        outer *= s
+    with _on(state.device, state, parents):
+        if nbytes and outer and B and N > 1:
+            X.check(X.lib().t2s_beam_reorder(state.data_ptr(), parents.contiguous().data_ptr(), outer, B, N, row, nbytes, X.stream()), "t2s_beam_reorder")
+    return state

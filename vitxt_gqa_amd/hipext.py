@@ -15,6 +15,8 @@ LIB_PATH = os.environ.get("T2S_HIP_LIB") or os.path.join(_HERE, "libt2s_hip.so")
 ABI_VERSION = 6
 
 T2S_F32, T2S_BF16 = 0, 1
+T2S_KV_INT8, T2S_KV_E4M3 = 0, 1
+T2S_BEAM_MAX = 32
 
 _SIGS = {
     "t2s_abi_version": (c_int, []),
@@ -63,6 +65,15 @@ _SIGS = {
     "t2s_gemm_nt": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_int] + [c_void_p] * 5),
     "t2s_gemm_wgrad_splits": (c_int, [c_int64, c_int, c_int]),
     "t2s_gemm_wgrad": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "t2s_kv8_append": (c_int, [c_void_p] + [c_int64] * 3 + [c_void_p] + [c_int64] * 3 + [c_void_p, c_int64] + [c_void_p] * 7 + [c_int] * 7 + [c_void_p]),
+    "t2s_kv8_dequantize": (c_int, [c_void_p] * 7 + [c_int] * 5 + [c_void_p]),
+    "t2s_kv8_attn_splits": (c_int, [c_int] * 5),
+    "t2s_kv8_attn_workspace_bytes": (c_int64, [c_int] * 5),
+    "t2s_kv8_attn": (c_int, [c_void_p] + [c_int64] * 3 + [c_void_p] * 7 + [c_int64] * 4 + [c_void_p, c_int64, c_int64, c_int] + [c_void_p] * 3 + [c_int64]
+                     + [c_int] * 6 + [c_float, c_int, c_int, c_void_p]),
+    "t2s_beam_select_workspace_bytes": (c_int64, [c_int] * 4),
+    "t2s_beam_select": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_int64] + [c_int] * 5 + [c_void_p]),
+    "t2s_beam_reorder": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int64, c_int64, c_void_p]),
 }
 
 _lib = None
