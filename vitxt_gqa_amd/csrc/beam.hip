@@ -32,21 +32,51 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
 // NaN counts as a masked word, +inf as the largest number
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
 
+// VEC consecutive logits; past the row's end: -inf.  `whole`: rows that start at 16-byte boundaries.
+template <typename TX, int VEC>
+__device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v, int V, bool whole, float* o) {
+  if (whole && v + VEC <= V) {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4) {
+      const f32x4 f = Vec4<TX>::load(x + v + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i + j] = clean(f[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o[i] = v + i < V ? clean((float)x[v + i]) : -INFINITY;
+  }
+}
+
+// a bound that the K largest of a wave's 64 keys reach and, where keys are unique, no others do; 1 where fewer than K are not zero.  Bit by
+// bit from the top, the lanes at or above a trial value counted by a ballot; done as soon as exactly K are left (some 20 steps on
+// random logits, 64 at most)
+__device__ __forceinline__ uint64_t wave_kth(uint64_t key, int K) {
+  uint64_t t = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t trial = t | 1ull << bit;
+    const int c = __popcll(__ballot(key >= trial));
+    if (c >= K) t = trial;
+    if (c == K) break;
+  }
+  return t ? t : 1;
+}
+
 template <typename TX>
 __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ logits, int64_t l_bs, int64_t l_ns, const float* __restrict__ cum,
                                                         const uint8_t* __restrict__ finished, uint64_t* __restrict__ keys, double* __restrict__ sums,
                                                         float* __restrict__ maxs, int N, int V, int K, int pad, int chunks, int subs) {
-  __shared__ uint64_t best_s[256];
-  __shared__ uint64_t list_s[BS_MAX * (BS_EPT + 1)];
-  __shared__ uint64_t top_s[BS_MAX];
-  __shared__ uint64_t thr_s;
-  __shared__ int cnt_s;
+  constexpr int VEC = 16 / sizeof(TX), SEG = BS_MAX * (BS_EPT + 1);
+  __shared__ uint64_t list_s[4][SEG];
+  __shared__ uint64_t top_s[BS_MAX], thr_s[4];
+  __shared__ int cnt_s[4];
   __shared__ float m_s[4];
   __shared__ double s_s[4];
-  const int tid = threadIdx.x, chunk = blockIdx.x % chunks;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, chunk = blockIdx.x % chunks;
   const int64_t row = blockIdx.x / chunks;
   const int b = (int)(row / N), n = (int)(row % N);
   const TX* x = logits + (int64_t)b * l_bs + (int64_t)n * l_ns;
+  const bool whole = (uintptr_t)x % 16 == 0;
   const float c = cum[row];
   const bool dead = !(c > -INFINITY);                                  // -inf or NaN: every candidate of the row is -inf
   const bool ended = finished && finished[row];
@@ -60,25 +90,28 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     if (v0 >= V) break;
     // of a row without logits only its first words (all -inf, lowest index first) and `pad` can be selected
     if (virt && sub != 0 && !(only >= v0 && only < v0 + BS_SUB)) continue;
-    uint64_t key[BS_EPT];
     float val[BS_EPT];
-    float mx = -INFINITY;
-    uint64_t best = 0;
 #pragma unroll
-    for (int i = 0; i < BS_EPT; ++i) {
-      const int64_t v = v0 + i * 256 + tid;
-      val[i] = -INFINITY;
-      if (v < V) {
-        if (!virt) val[i] = clean((float)x[v]);
-        else if (v == only) val[i] = 0.f;
+    for (int i = 0; i < BS_EPT; i += VEC) {
+      const int64_t v = v0 + i * 256 + tid * VEC;
+      if (!virt) {
+        load_logits<TX, VEC>(x, v, V, whole, val + i);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) val[i + j] = v + j == only ? 0.f : -INFINITY;
       }
-      key[i] = v < V ? (uint64_t)ordered(val[i]) << 32 | (0xffffffffu - (uint32_t)v) : 0;
     }
+    auto index = [&](int i) { return v0 + (i / VEC) * VEC * 256 + tid * VEC + i % VEC; };       // rises with i
+    auto key_of = [&](float x, int64_t v) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - (uint32_t)v); };
+    float mx = val[0];
+    int at = 0;
 #pragma unroll
-    for (int i = 0; i < BS_EPT; ++i) {
-      mx = fmaxf(mx, val[i]);
-      best = key[i] > best ? key[i] : best;
-    }
+    for (int i = 1; i < BS_EPT; ++i)
+      if (val[i] > mx) {
+        mx = val[i];
+        at = i;
+      }
+    uint64_t best = index(0) < V ? key_of(mx, index(at)) : 0;
     if (mx > m) {
       sum *= (double)__expf(m - mx);
       m = mx;
@@ -89,37 +122,46 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
       for (int i = 0; i < BS_EPT; ++i) s += __expf(val[i] - m);
       sum += (double)s;
     }
-    // ---- the K best of (this stretch, what is kept of the former ones).  The K-th largest of the threads' best keys bounds the K-th
-    // largest key from below, and only the K threads at or above it hold keys that count: at most K (BS_EPT + 1) of them.
+    // ---- the K best of (this stretch, what is kept of the former ones).  The K-th largest of a wave's best keys, one a lane, bounds the
+    // stretch's K-th largest key from below; so does the largest such bound of the four waves.  Of a wave's lanes at most K reach its own
+    // bound, so at most K (BS_EPT + 1) of its keys are listed - on random logits hardly more than K of all four.
     __syncthreads();
     const uint64_t kept = tid < K ? top_s[tid] : 0;
     best = kept > best ? kept : best;
-    best_s[tid] = best;
-    if (tid == 0) {
-      thr_s = 1;
-      cnt_s = 0;
-    }
+    const uint64_t own = wave_kth(best, K);
+    if (lane == 0) thr_s[wave] = own;
     __syncthreads();
-    if (best) {
-      int rank = 0;
-#pragma unroll 16
-      for (int i = 0; i < 256; ++i) rank += best_s[i] > best;
-      if (rank == K - 1) thr_s = best;
-    }
-    __syncthreads();
-    const uint64_t thr = thr_s;
-    if (best >= thr) {
+    uint64_t thr = thr_s[0];
 #pragma unroll
-      for (int i = 0; i < BS_EPT; ++i)
-        if (key[i] >= thr) list_s[atomicAdd(&cnt_s, 1)] = key[i];
-      if (kept >= thr) list_s[atomicAdd(&cnt_s, 1)] = kept;
-    }
+    for (int w = 1; w < 4; ++w) thr = thr_s[w] > thr ? thr_s[w] : thr;
+    // (a bound found early is the upper bits of a key: below those of -inf it is no number, and everything passes)
+    const float tv = thr >> 32 > 0x7fffffu ? from_ordered((uint32_t)(thr >> 32)) : -INFINITY;
+    int cnt = 0;                                                        // of this wave
+#pragma unroll
+    for (int i = 0; i < BS_EPT; ++i)
+      if (__ballot(val[i] >= tv)) {
+        const uint64_t k = key_of(val[i], index(i));
+        const bool in = index(i) < V && k >= thr;
+        const uint64_t who = __ballot(in);
+        if (in) list_s[wave][cnt + __popcll(who & ((1ull << lane) - 1))] = k;
+        cnt += __popcll(who);
+      }
+    const uint64_t who = __ballot(kept >= thr);
+    if (kept >= thr) list_s[wave][cnt + __popcll(who & ((1ull << lane) - 1))] = kept;
+    cnt += __popcll(who);
+    if (lane == 0) cnt_s[wave] = cnt;
     __syncthreads();
-    const int cnt = cnt_s;
-    for (int i = tid; i < cnt; i += 256) {
-      const uint64_t mine = list_s[i];
+    const int c0 = cnt_s[0], c1 = c0 + cnt_s[1], c2 = c1 + cnt_s[2], c3 = c2 + cnt_s[3];
+    for (int i = tid; i < c3; i += 256) {
+      const int w = (i >= c0) + (i >= c1) + (i >= c2);
+      const uint64_t mine = list_s[w][i - (w == 0 ? 0 : w == 1 ? c0 : w == 2 ? c1 : c2)];
       int rank = 0;
-      for (int j = 0; j < cnt; ++j) rank += list_s[j] > mine;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int n_u = u == 0 ? c0 : u == 1 ? c1 - c0 : u == 2 ? c2 - c1 : c3 - c2;
+#pragma unroll 4
+        for (int j = 0; j < n_u; ++j) rank += list_s[u][j] > mine;
+      }
       if (rank < K) top_s[rank] = mine;
     }
   }
@@ -127,7 +169,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
   float mw = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mw = fmaxf(mw, __shfl_xor(mw, o, 64));
-  double sw = m > -INFINITY ? sum * exp((double)m - (double)mw) : 0.0;
+  double sw = m > -INFINITY ? sum * (double)__expf(m - mw) : 0.0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sw += __shfl_xor(sw, o, 64);
   if ((tid & 63) == 0) {
@@ -141,92 +183,112 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     const float m4 = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
     double s4 = 0.0;
     for (int w = 0; w < 4; ++w)
-      if (m_s[w] > -INFINITY) s4 += s_s[w] * exp((double)m_s[w] - (double)m4);
+      if (m_s[w] > -INFINITY) s4 += s_s[w] * (double)__expf(m_s[w] - m4);
     maxs[at] = m4;
     sums[at] = s4;
   }
 }
 
-struct Cand {
+struct __attribute__((aligned(16))) Cand {
   double score;
-  int64_t flat;       // n V + v; INT64_MAX: no candidate
+  int64_t flat;       // n << 32 | v, in the order of n V + v; INT64_MAX: no candidate
 };
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
 
-// one workgroup per sequence: joins the stretches, orders the N rows' candidates
+constexpr int BJ_PER = 4;                          // candidates of a thread at a time
+
+// order-preserving unsigned form of a double, never 0
+__device__ __forceinline__ uint64_t ordered64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// one workgroup per sequence: joins the stretches, orders the N rows' candidates, 256 BJ_PER of them at a time
 __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restrict__ keys, const double* __restrict__ sums, const float* __restrict__ maxs,
                                                         const float* __restrict__ cum, const uint8_t* __restrict__ finished, float* __restrict__ out_scores,
-                                                        int64_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens, int N, int V, int K, int chunks) {
-  __shared__ double off_s[BS_MAX], score_s[256];
+                                                        int64_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens, int N, int K, int chunks) {
+  __shared__ double off_s[BS_MAX];
   __shared__ float top_m[BS_MAX];
-  __shared__ int64_t flat_s[256];
-  __shared__ int list_s[BS_MAX * BS_MAX * BS_CHUNKS * BS_MAX / 256];
+  __shared__ Cand list_s[256 * BJ_PER + BS_MAX], top_s[BS_MAX];
+  __shared__ uint64_t thr_s[4];
   __shared__ int cnt_s;
-  __shared__ Cand thr_s;
-  const int tid = threadIdx.x, b = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.x;
+  const int per_row = chunks * K, M = N * per_row;                     // (32 * 32 * 32 at most)
+  const float per_inv = 1.0f / (float)per_row;
+  const Cand none{-INFINITY, INT64_MAX};
+  const uint64_t* kb = keys + (int64_t)b * M;
+  uint64_t raw[BJ_PER];                            // (in flight beside the rows' sums)
+#pragma unroll
+  for (int j = 0; j < BJ_PER; ++j) raw[j] = tid + j * 256 < M ? kb[tid + j * 256] : 0;
   if (tid < N) {
     const int64_t row = (int64_t)b * N + tid;
     const float c = cum[row];
-    float m = -INFINITY;
-    for (int i = 0; i < chunks; ++i) m = fmaxf(m, maxs[row * chunks + i]);
-    double s = 0.0;
-    for (int i = 0; i < chunks; ++i) {
-      const float mi = maxs[row * chunks + i];
-      if (mi > -INFINITY) s += sums[row * chunks + i] * exp((double)mi - (double)m);
-    }
     const bool ended = finished && finished[row];
+    float m = -INFINITY;
+    double s = 0.0;
+#pragma unroll 4
+    for (int i = 0; i < chunks; ++i) {
+      const float mi = maxs[row * chunks + i], mn = fmaxf(m, mi);
+      const double si = sums[row * chunks + i];
+      if (mn > -INFINITY) s = s * (double)__expf(m - mn) + si * (double)__expf(mi - mn);
+      m = mn;
+    }
     const double cd = c > -INFINITY ? (double)fminf(c, 3.402823466e38f) : -INFINITY;
     top_m[tid] = ended ? 0.f : m;
     off_s[tid] = ended || !(s > 0.0) ? cd : cd - log(s);
   }
-  if (tid == 0) {
-    cnt_s = 0;
-    thr_s = Cand{-INFINITY, INT64_MAX};
-  }
+  if (tid < K) top_s[tid] = none;
   __syncthreads();
-  const int M = N * chunks * K;
-  const uint64_t* kb = keys + (int64_t)b * M;
-  auto cand = [&](int i) {
-    const uint64_t k = kb[i];
-    const int n = i / (chunks * K);
-    if (!k) return Cand{-INFINITY, INT64_MAX};
-    const float x = from_ordered((uint32_t)(k >> 32));
-    const double sc = x > -INFINITY ? off_s[n] + ((double)x - (double)top_m[n]) : -INFINITY;
-    return Cand{sc, (int64_t)n * V + (0xffffffffu - (uint32_t)k)};
-  };
-  Cand best{-INFINITY, INT64_MAX};
-  for (int i = tid; i < M; i += 256) {
-    const Cand c = cand(i);
-    if (before(c, best)) best = c;
-  }
-  score_s[tid] = best.score;
-  flat_s[tid] = best.flat;
-  __syncthreads();
-  if (best.flat != INT64_MAX) {
-    int rank = 0;
-    for (int i = 0; i < 256; ++i) rank += before(Cand{score_s[i], flat_s[i]}, best);
-    if (rank == K - 1) thr_s = best;
-  }
-  __syncthreads();
-  const Cand thr = thr_s;
-  // the K best are among the candidates that do not come behind `thr`: those of at most K threads
-  if (best.flat != INT64_MAX && !before(thr, best))
-    for (int i = tid; i < M; i += 256) {
-      const Cand c = cand(i);
-      if (c.flat != INT64_MAX && !before(thr, c)) list_s[atomicAdd(&cnt_s, 1)] = i;
+  for (int m0 = 0; m0 < M; m0 += 256 * BJ_PER) {
+    Cand c[BJ_PER];
+    const Cand kept = tid < K ? top_s[tid] : none;
+    uint64_t best = kept.flat != INT64_MAX ? ordered64(kept.score) : 0;
+#pragma unroll
+    for (int j = 0; j < BJ_PER; ++j) {
+      const int i = m0 + tid + j * 256;
+      const uint64_t k = m0 == 0 ? raw[j] : (i < M ? kb[i] : 0);
+      c[j] = none;
+      if (k) {
+        const int n = (int)(((float)i + 0.5f) * per_inv);              // i / per_row: half a step from every border, 2^-23 relative off
+        const float x = from_ordered((uint32_t)(k >> 32));
+        c[j].score = x > -INFINITY ? off_s[n] + ((double)x - (double)top_m[n]) : -INFINITY;
+        c[j].flat = (int64_t)n << 32 | (0xffffffffu - (uint32_t)k);
+        best = max(best, ordered64(c[j].score));
+      }
     }
-  __syncthreads();
-  const int cnt = cnt_s;
-  for (int i = tid; i < cnt; i += 256) {
-    const Cand mine = cand(list_s[i]);
-    int rank = 0;
-    for (int j = 0; j < cnt; ++j) rank += before(cand(list_s[j]), mine);
-    if (rank < K) {
-      const int64_t at = (int64_t)b * K + rank;
-      out_scores[at] = (float)mine.score;
-      out_parents[at] = mine.flat / V;
-      out_tokens[at] = mine.flat % V;
+    // a lower bound for the K-th best score, as in the rows' kernel; equal scores are all listed (the list holds everything there is)
+    if (tid == 0) cnt_s = 0;
+    uint64_t thr = 1;
+    if (M > 256) {
+      thr = wave_kth(best, K);
+      if (lane == 0) thr_s[tid >> 6] = thr;
     }
+    __syncthreads();
+    if (M > 256)
+      for (int w = 0; w < 4; ++w) thr = max(thr, thr_s[w]);
+    if (best >= thr) {
+#pragma unroll
+      for (int j = 0; j < BJ_PER; ++j)
+        if (c[j].flat != INT64_MAX && ordered64(c[j].score) >= thr) list_s[atomicAdd(&cnt_s, 1)] = c[j];
+      if (kept.flat != INT64_MAX && ordered64(kept.score) >= thr) list_s[atomicAdd(&cnt_s, 1)] = kept;
+    }
+    __syncthreads();
+    const int cnt = cnt_s;
+    for (int i = tid; i < cnt; i += 256) {
+      const Cand mine = list_s[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < cnt; ++j) rank += before(list_s[j], mine);
+      if (rank < K) top_s[rank] = mine;
+    }
+    __syncthreads();
+  }
+  if (tid < K) {
+    const Cand r = top_s[tid];
+    const int64_t at = (int64_t)b * K + tid;
+    out_scores[at] = (float)r.score;
+    out_parents[at] = r.flat >> 32;
+    out_tokens[at] = r.flat & 0xffffffff;
   }
 }
 
@@ -312,7 +374,7 @@ extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t
     hipLaunchKernelGGL(beam_rows_kernel<float>, dim3((unsigned)grid), dim3(256), 0, st, (const float*)logits, batch_stride, beam_stride, scores, finished, keys, sums, maxs,
                        N, V, n_select, pad, chunks, subs);
   T2S_CHECK_LAUNCH("beam_select");
-  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)B), dim3(256), 0, st, keys, sums, maxs, scores, finished, out_scores, out_parents, out_tokens, N, V, n_select, chunks);
+  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)B), dim3(256), 0, st, keys, sums, maxs, scores, finished, out_scores, out_parents, out_tokens, N, n_select, chunks);
   T2S_CHECK_LAUNCH("beam_join");
   return 0;
 }
