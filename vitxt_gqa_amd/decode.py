@@ -12,7 +12,8 @@ runs it on these operators (t2s.py ``_beam_decode``); they are also usable on th
 Thin wrappers over the C ABI (``include/t2s_hip.h``; kernels in ``csrc/kv8.hip`` and ``csrc/beam.hip``): shapes, types, strides and devices are
 checked on the host, everything runs on the current stream of the tensors' device, without a synchronisation and without state other than
 the cache's own tensors - a step may be captured into a graph.  No gradients: the operands may not require any."""
-import contextlib
+import functools
+import math
 
 import torch
 
@@ -22,7 +23,7 @@ BLOCK = 64                  # tokens of a block: one scale for its keys and one 
 HEAD_DIM = 64
 BEAM_MAX = X.T2S_BEAM_MAX   # beams, and candidates a selection returns
 FORMATS = {"int8": (X.T2S_KV_INT8, torch.int8), "e4m3": (X.T2S_KV_E4M3, torch.float8_e4m3fn)}
-_NULL = contextlib.nullcontext()
+_DTYPES = {torch.float32: (X.T2S_F32, 15), torch.bfloat16: (X.T2S_BF16, 7)}          # code, mask of a 4-element alignment in bytes
 
 
 def _need(ok, msg, *args):
@@ -30,23 +31,48 @@ def _need(ok, msg, *args):
         raise ValueError(msg % args if args else msg)
 
 
-def _on(device, *tensors):
-    """All of ``tensors`` (None: absent) on ``device``, a GPU; returns the context in which its current stream is the one to launch on."""
-    if device.type != "cuda":
-        raise RuntimeError("T2S HIP kernels need device tensors (got a %s tensor); there is no CPU path" % device)
+def _same_device(index, *tensors):
+    """All of ``tensors`` (None: absent) on GPU ``index`` and without gradients."""
     for t in tensors:
-        if t is not None:
-            _need(t.device == device, "tensors on %s and %s: all of a call's tensors live on one device", device, t.device)
-            _need(not (t.requires_grad and torch.is_grad_enabled()), "the decode operators have no gradients: call them under torch.no_grad() or on detached tensors")
-    return _NULL if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        if t is not None and (t.get_device() != index or index < 0 or t.requires_grad):
+            if index < 0 or t.get_device() < 0:
+                _need(index < 0, "tensors on %s and cuda:%d: all of a call's tensors live on one device", t.device, index)
+                raise RuntimeError("T2S HIP kernels need device tensors (got a %s tensor); there is no CPU path" % t.device)
+            _need(t.get_device() == index, "tensors on %s and cuda:%d: all of a call's tensors live on one device", t.device, index)
+            _need(not torch.is_grad_enabled(), "the decode operators have no gradients: call them under torch.no_grad() or on detached tensors")
+
+
+def _launch(index, fn, *args):
+    """fn(*args, stream) on the current stream of GPU ``index``."""
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _head_rows(t, name):
-    """[..., heads, 64] with dense 64-element rows that start at multiples of 4 elements."""
-    _need(t.dtype in (torch.bfloat16, torch.float32), "%s: float32 or bfloat16, got %s", name, t.dtype)
-    _need(t.shape[-1] == HEAD_DIM, "%s: the kernels are built for head_dim 64, got %s", name, tuple(t.shape))
-    ok = t.stride(-1) == 1 and t.data_ptr() % (4 * t.element_size()) == 0 and not any(s % 4 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
-    _need(ok, "%s: rows of 64 dense elements, aligned to 4 elements, are needed (strides %s): call .contiguous()", name, t.stride())
+    """Strides of [..., heads, 64] with dense 64-element rows that start at multiples of 4 elements (0 for axes of length 1)."""
+    s = t.stride()
+    d = _DTYPES.get(t.dtype)
+    if d is None or t.shape[-1] != HEAD_DIM or s[-1] != 1 or t.data_ptr() & d[1] or any([x & 3 for x in s[:-1]]):
+        _need(d is not None, "%s: float32 or bfloat16, got %s", name, t.dtype)
+        _need(t.shape[-1] == HEAD_DIM, "%s: the kernels are built for head_dim 64, got %s", name, tuple(t.shape))
+        s = tuple(x if n > 1 else 0 for x, n in zip(s[:-1], t.shape[:-1])) + (s[-1],)
+        _need(s[-1] == 1 and not t.data_ptr() & d[1] and not any(x & 3 for x in s[:-1]),
+              "%s: rows of 64 dense elements, aligned to 4 elements, are needed (strides %s): call .contiguous()", name, t.stride())
+    return s
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_plan(B, N, H, G, max_len):
+    """(shares of the token axis, bytes of workspace) of an attention over about ``max_len`` tokens."""
+    splits = X.lib().t2s_kv8_attn_splits(B, N, H, G, max_len)
+    return splits, X.lib().t2s_kv8_attn_workspace_bytes(B, N, H, G, splits)
+
+
+@functools.lru_cache(maxsize=256)
+def _select_bytes(B, N, V, K):
+    return X.lib().t2s_beam_select_workspace_bytes(B, N, V, K)
 
 
 class KVCache8:
@@ -95,6 +121,8 @@ class KVCache8:
         self.batch, self.heads, self.blocks, self.capacity, self.device = B, H, n, n * BLOCK, k.device
         self.max_len = self.capacity if max_len is None else min(int(max_len), self.capacity)
         self._ticket = torch.zeros(B, dtype=torch.int32, device=k.device)
+        self._index = k.get_device()
+        self._ptrs, self._ticket_ptr = tuple(t.data_ptr() for t in (k, v, ks, vs, lens)), self._ticket.data_ptr()
 
     def append(self, k, v, counts=None, rows=None):
         """Puts new tokens behind what each sequence holds.  k, v: [B, R, H, 64] float32 or bfloat16, dense 64-element rows (slices of a fused
@@ -105,28 +133,27 @@ class KVCache8:
         A block that holds tokens already keeps the larger of its scale and the new tokens' one; its codes are rounded again where it grew.
         A value that is not finite, or a row number outside 0 .. R - 1, turns its block of that head to NaN.  Tokens that do not fit turn the
         sequence's length to -1 and every result over it to NaN, until ``set_lens`` (the lengths live on the device: nothing is waited for)."""
-        _need(k.dim() == 4 and k.shape[0] == self.batch and k.shape[2] == self.heads and v.shape == k.shape and v.dtype == k.dtype,
-              "append: k and v [%d, R, %d, 64] of one type, got %s %s and %s %s", self.batch, self.heads, tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
-        R = k.shape[1]
-        T = R
+        B, H = self.batch, self.heads
+        if k.dim() != 4 or k.shape[0] != B or k.shape[2] != H or v.shape != k.shape or v.dtype != k.dtype:
+            _need(False, "append: k and v [%d, R, %d, 64] of one type, got %s %s and %s %s", B, H, tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
+        R = T = k.shape[1]
+        rp, rs, cp = None, 0, None
         if rows is not None:
-            _need(rows.dim() == 2 and rows.shape[0] == self.batch and rows.dtype == torch.int32 and (rows.shape[1] < 2 or rows.stride(1) == 1),
-                  "append: rows is int32 [%d, T] with dense rows, got %s %s", self.batch, tuple(rows.shape), rows.dtype)
-            T = rows.shape[1]
+            _need(rows.dim() == 2 and rows.shape[0] == B and rows.dtype == torch.int32 and (rows.shape[1] < 2 or rows.stride(1) == 1),
+                  "append: rows is int32 [%d, T] with dense rows, got %s %s", B, tuple(rows.shape), rows.dtype)
+            T, rp, rs = rows.shape[1], rows.data_ptr(), rows.stride(0)
         if counts is not None:
-            _need(counts.shape == (self.batch,) and counts.dtype == torch.int32 and counts.is_contiguous(), "append: counts is a dense int32 [%d]", self.batch)
-        _need(counts is not None or T <= self.capacity, "append: %d tokens do not fit a capacity of %d", T, self.capacity)
+            _need(counts.shape == (B,) and counts.dtype == torch.int32 and (B == 1 or counts.stride(0) == 1), "append: counts is a dense int32 [%d]", B)
+            cp = counts.data_ptr()
+        elif T > self.capacity:
+            _need(False, "append: %d tokens do not fit a capacity of %d", T, self.capacity)
         _need(R > 0 or T == 0, "append: %d tokens of no rows", T)
-        if T:
-            _head_rows(k, "append: k")
-            _head_rows(v, "append: v")
-        with _on(self.device, k, v, counts, rows):
-            if T == 0:
-                return self
-            X.check(X.lib().t2s_kv8_append(k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], None if rows is None else rows.data_ptr(),
-                                           0 if rows is None else rows.stride(0), None if counts is None else counts.data_ptr(), self.k.data_ptr(), self.v.data_ptr(),
-                                           self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.lens.data_ptr(), self._ticket.data_ptr(),
-                                           self.batch, self.heads, T, R, self.blocks, X.dtype_code(k), self._fmt, X.stream()), "t2s_kv8_append")
+        sk, sv = (_head_rows(k, "append: k"), _head_rows(v, "append: v")) if T else (None, None)
+        _same_device(self._index, k, v, counts, rows)
+        if T == 0:
+            return self
+        X.check(_launch(self._index, X.lib().t2s_kv8_append, k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], rp, rs, cp, *self._ptrs,
+                        self._ticket_ptr, B, H, T, R, self.blocks, _DTYPES[k.dtype][0], self._fmt), "t2s_kv8_append")
         self.max_len = min(self.capacity, self.max_len + T)
         return self
 
@@ -148,10 +175,10 @@ class KVCache8:
     def dequantize(self, dtype=torch.bfloat16):
         """(keys, values) [B, H, capacity, 64] in ``dtype`` (float32 or bfloat16): code * scale, zeros behind a sequence's length."""
         _need(dtype in (torch.bfloat16, torch.float32), "dequantize: float32 or bfloat16, got %s", dtype)
-        with _on(self.device):
-            k, v = (torch.empty(self.batch, self.heads, self.capacity, HEAD_DIM, dtype=dtype, device=self.device) for _ in range(2))
-            X.check(X.lib().t2s_kv8_dequantize(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), self.lens.data_ptr(),
-                                               k.data_ptr(), v.data_ptr(), self.batch, self.heads, self.blocks, X.dtype_code(k), self._fmt, X.stream()), "t2s_kv8_dequantize")
+        _same_device(self._index, self.k)
+        k, v = (torch.empty(self.batch, self.heads, self.capacity, HEAD_DIM, dtype=dtype, device=self.device) for _ in range(2))
+        X.check(_launch(self._index, X.lib().t2s_kv8_dequantize, *self._ptrs, k.data_ptr(), v.data_ptr(), self.batch, self.heads, self.blocks,
+                        _DTYPES[dtype][0], self._fmt), "t2s_kv8_dequantize")
         return k, v
 
 
@@ -166,41 +193,38 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
 
     Codes enter the matrix pipe as exact bf16; a query in float32 as the three bf16 terms that make it up; probabilities as two terms (bfloat16
     results: 16 bits, below the rounding of the result) or three (float32).  All sums, maxima and scales are float32; the result is rounded once."""
-    _need(q.dim() == 4 and q.shape[0] == cache.batch and q.shape[2] > 0 and q.shape[2] % cache.heads == 0,
-          "attend: q [%d, N, a multiple of %d, 64], got %s", cache.batch, cache.heads, tuple(q.shape))
+    H = cache.heads
+    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[2] < 1 or q.shape[2] % H:
+        _need(False, "attend: q [%d, N, a multiple of %d, 64], got %s", cache.batch, H, tuple(q.shape))
     B, N, HQ, _ = q.shape
-    T, tk, tv, ts, tl, tls = 0, None, None, (0, 0, 0, 0), None, (0, 0)
-    _need((tail_k is None) == (tail_v is None), "attend: tail_k and tail_v come together")
-    _head_rows(q, "attend: q")
-    if tail_k is not None:
+    sq = _head_rows(q, "attend: q")
+    T, tk, tv, st, tl, tls = 0, None, None, (0, 0, 0, 0), None, (0, 0)
+    if tail_k is not None and tail_v is not None:
         T = tail_k.shape[2] if tail_k.dim() == 5 else -1
-        _need(tuple(tail_k.shape) == (B, N, T, cache.heads, HEAD_DIM) and tail_v.shape == tail_k.shape and tail_k.dtype == q.dtype and tail_v.dtype == q.dtype,
-              "attend: tails [%d, %d, T, %d, 64] of q's type, got %s %s and %s %s", B, N, cache.heads, tuple(tail_k.shape), tail_k.dtype, tuple(tail_v.shape), tail_v.dtype)
+        if tail_k.shape != (B, N, T, H, HEAD_DIM) or tail_v.shape != tail_k.shape or tail_k.dtype != q.dtype or tail_v.dtype != q.dtype:
+            _need(False, "attend: tails [%d, %d, T, %d, 64] of q's type, got %s %s and %s %s", B, N, H, tuple(tail_k.shape), tail_k.dtype, tuple(tail_v.shape), tail_v.dtype)
         if torch.is_tensor(tail_len):
             _need(tail_len.shape == (B, N) and tail_len.dtype == torch.int32, "attend: tail_len is an int or int32 [%d, %d]", B, N)
-            tl, tls = tail_len, tail_len.stride()
+            tl, tls = tail_len.data_ptr(), tail_len.stride()
         elif tail_len is not None:
             T = max(0, min(int(tail_len), T))
         if T > 0:
-            _head_rows(tail_k, "attend: tail_k")
-            _head_rows(tail_v, "attend: tail_v")
-            _need(tail_k.stride() == tail_v.stride(), "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
-            tk, tv, ts = tail_k.data_ptr(), tail_v.data_ptr(), tail_k.stride()[:4]
+            st = _head_rows(tail_k, "attend: tail_k")
+            if _head_rows(tail_v, "attend: tail_v") != st:
+                _need(False, "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
+            tk, tv = tail_k.data_ptr(), tail_v.data_ptr()
     else:
+        _need(tail_k is None and tail_v is None, "attend: tail_k and tail_v come together")
         _need(tail_len is None, "attend: tail_len without a tail")
-    with _on(cache.device, q, tail_k, tail_v, tl):
-        out = torch.empty(B, N, HQ, HEAD_DIM, dtype=q.dtype, device=q.device)
-        lse = torch.empty(B, N, HQ, dtype=torch.float32, device=q.device)
-        if N == 0:
-            return out, lse
-        G = HQ // cache.heads
-        lib = X.lib()
-        splits = lib.t2s_kv8_attn_splits(B, N, cache.heads, G, cache.max_len)
-        nbytes = lib.t2s_kv8_attn_workspace_bytes(B, N, cache.heads, G, splits)
-        ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
-        X.check(lib.t2s_kv8_attn(q.data_ptr(), *q.stride()[:3], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-                                 cache.lens.data_ptr(), tk, tv, *ts, None if tl is None else tl.data_ptr(), *tls, T, out.data_ptr(), lse.data_ptr(),
-                                 ws.data_ptr(), nbytes, splits, B, N, cache.heads, G, cache.blocks, float(scale), X.dtype_code(q), cache._fmt, X.stream()), "t2s_kv8_attn")
+    _same_device(cache._index, q, tail_k, tail_v, None if tl is None else tail_len)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, N, HQ), dtype=torch.float32, device=q.device)
+    if N == 0:
+        return out, lse
+    splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+    X.check(_launch(cache._index, X.lib().t2s_kv8_attn, q.data_ptr(), sq[0], sq[1], sq[2], *cache._ptrs, tk, tv, st[0], st[1], st[2], st[3], tl, tls[0], tls[1], T,
+                    out.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, _DTYPES[q.dtype][0], cache._fmt), "t2s_kv8_attn")
     return out, lse
 
 
@@ -212,29 +236,35 @@ def beam_select(logits, scores, n_select, finished=None, pad=0):
     ``finished`` bool [B, N]: a beam that has ended offers the token ``pad`` at its own score and nothing else.  NaN logits count as -inf, +inf as
     the largest number.  Returns (scores [B, n_select] float32, parents int64: the beam n, tokens int64: the word v), best first, ties to the lowest
     n V + v; candidates at -inf only where nothing else is left.  At most 32 beams and 32 candidates."""
-    _need(logits.dim() == 3 and logits.shape[2] > 0 and logits.shape[1] > 0, "beam_select: logits [B, N, V], got %s", tuple(logits.shape))
+    if logits.dim() != 3 or logits.shape[2] < 1 or logits.shape[1] < 1:
+        _need(False, "beam_select: logits [B, N, V], got %s", tuple(logits.shape))
     B, N, V = logits.shape
     K = int(n_select)
-    _need(logits.dtype in (torch.bfloat16, torch.float32), "beam_select: float32 or bfloat16 logits, got %s", logits.dtype)
-    _need(V == 1 or logits.stride(2) == 1, "beam_select: dense rows of logits are needed (strides %s): call .contiguous()", logits.stride())
-    _need(scores.shape == (B, N) and scores.dtype == torch.float32, "beam_select: scores is float32 [%d, %d], got %s %s", B, N, tuple(scores.shape), scores.dtype)
-    _need(N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V, "beam_select: %d of %d x %d candidates (at most %d beams and %d candidates)", K, N, V, BEAM_MAX, BEAM_MAX)
-    _need(0 <= pad < V, "beam_select: pad %d outside the vocabulary of %d", pad, V)
+    d = _DTYPES.get(logits.dtype)
+    if d is None or scores.shape != (B, N) or scores.dtype != torch.float32 or (V > 1 and logits.stride(2) != 1):
+        _need(d is not None, "beam_select: float32 or bfloat16 logits, got %s", logits.dtype)
+        _need(V == 1 or logits.stride(2) == 1, "beam_select: dense rows of logits are needed (strides %s): call .contiguous()", logits.stride())
+        _need(False, "beam_select: scores is float32 [%d, %d], got %s %s", B, N, tuple(scores.shape), scores.dtype)
+    if not (N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V and 0 <= pad < V):
+        _need(N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V, "beam_select: %d of %d x %d candidates (at most %d beams and %d candidates)", K, N, V, BEAM_MAX, BEAM_MAX)
+        _need(False, "beam_select: pad %d outside the vocabulary of %d", pad, V)
+    fp = None
     if finished is not None:
-        _need(finished.shape == (B, N) and finished.dtype in (torch.bool, torch.uint8), "beam_select: finished is bool [%d, %d], got %s %s", B, N, tuple(finished.shape), finished.dtype)
-    with _on(logits.device, logits, scores, finished):
-        out = torch.empty(B, K, dtype=torch.float32, device=logits.device)
-        parents, tokens = torch.empty(2, B, K, dtype=torch.int64, device=logits.device).unbind(0)
-        if B == 0:
-            return out, parents, tokens
-        scores = scores.contiguous()
-        if finished is not None:
-            finished = finished.contiguous()
-        lib = X.lib()
-        nbytes = lib.t2s_beam_select_workspace_bytes(B, N, V, K)
-        ws = torch.empty((nbytes + 7) // 8, dtype=torch.int64, device=logits.device)
-        X.check(lib.t2s_beam_select(logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), None if finished is None else finished.data_ptr(), int(pad),
-                                    out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, X.dtype_code(logits), X.stream()), "t2s_beam_select")
+        if finished.shape != (B, N) or (finished.dtype != torch.bool and finished.dtype != torch.uint8):
+            _need(False, "beam_select: finished is bool [%d, %d], got %s %s", B, N, tuple(finished.shape), finished.dtype)
+        finished = finished.contiguous()
+        fp = finished.data_ptr()
+    index = logits.get_device()
+    _same_device(index, logits, scores, finished)
+    out = torch.empty((B, K), dtype=torch.float32, device=logits.device)
+    parents, tokens = torch.empty((2, B, K), dtype=torch.int64, device=logits.device).unbind(0)
+    if B == 0:
+        return out, parents, tokens
+    scores = scores.contiguous()
+    nbytes = _select_bytes(B, N, V, K)
+    ws = torch.empty((nbytes + 7) // 8, dtype=torch.int64, device=logits.device)
+    X.check(_launch(index, X.lib().t2s_beam_select, logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), fp, pad, out.data_ptr(), parents.data_ptr(),
+                    tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, d[0]), "t2s_beam_select")
     return out, parents, tokens
 
 
@@ -251,17 +281,15 @@ def beam_reorder(state, parents, batch_dim=0, used=None):
     _need(N <= BEAM_MAX, "beam_reorder: at most %d beams, got %d", BEAM_MAX, N)
     _need(parents.shape == (B, N) and parents.dtype == torch.int64, "beam_reorder: parents is int64 [%d, %d], got %s %s", B, N, tuple(parents.shape), parents.dtype)
     rest = state.shape[d + 2:]
-    row = state.element_size()
-    for s in rest:
-        row *= s
+    row = state.element_size() * math.prod(rest)
     nbytes = row
     if used is not None:
         _need(len(rest) > 0 and 0 <= used <= rest[0], "beam_reorder: used %s of %s", used, tuple(rest))
         nbytes = row // max(1, rest[0]) * int(used)
-    outer = 1
-    for s in state.shape[:d]:
-        outer *= s
-    with _on(state.device, state, parents):
-        if nbytes and outer and B and N > 1:
-            X.check(X.lib().t2s_beam_reorder(state.data_ptr(), parents.contiguous().data_ptr(), outer, B, N, row, nbytes, X.stream()), "t2s_beam_reorder")
+    outer = math.prod(state.shape[:d])
+    index = state.get_device()
+    _same_device(index, state, parents)
+    if nbytes and outer and B and N > 1:
+        parents = parents.contiguous()
+        X.check(_launch(index, X.lib().t2s_beam_reorder, state.data_ptr(), parents.data_ptr(), outer, B, N, row, nbytes), "t2s_beam_reorder")
     return state
