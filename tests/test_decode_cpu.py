@@ -115,7 +115,7 @@ def test_c_abi_refuses(lib):
         rc, err = append(**kw)
         assert rc != 0 and text in err, (kw, err)
     assert lib.t2s_kv8_dequantize(p, p, p, p, p, p, ctypes.c_void_p(8), 1, 1, 1, 0, 0, None) != 0 and b"alignment" in lib.t2s_last_error()
-    att = [p, 0, 64, 64, p, p, p, p, p, None, None, 0, 0, 0, 0, None, 0, 0, 0, p, p, p, 1 << 20, 1, 1, 1, 1, 1, 1, 0.125, 0, 0, None]
+    att = [p, 0, 64, 64, p, p, p, p, p, None, None, 0, 0, 0, 0, None, 0, 0, 0, p, p, p, 1 << 20, 2, 1, 1, 1, 1, 1, 0.125, 0, 0, None]
     for i, v, text in ((0, None, b"null pointer"), (24, 0, b"bad shape"), (9, p, b"come together"), (22, 8, b"too small"), (23, 0, b"too small"), (2, 63, b"aligned"), (30, 3, b"bad dtype"), (31, 3, b"bad format")):
         a = list(att)
         a[i] = v

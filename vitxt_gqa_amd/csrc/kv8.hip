@@ -259,10 +259,10 @@ struct AttnArgs {
   int tail_T;
   void* out;
   float* lse;
-  float* part_o;        // [B * H][nsplit][R][64]
-  float* part_ml;       // [B * H][nsplit][R][2]: running maximum (log2 units), sum
+  float* part_o;        // [B * H][nshare][R][64]
+  float* part_ml;       // [B * H][nshare][R][2]: running maximum (log2 units), sum
   float scale;
-  int B, N, H, G, nblk, nsplit, row_tiles;
+  int B, N, H, G, nblk, nsplit, nshare, row_tiles;      // nshare: nsplit shares of the cache, and one more for the tails where nsplit > 1
 };
 
 // x as a sum of TERMS bf16 numbers (8 significant bits each): 1 for what is bf16 already, 2 keep 16 bits, 3 the whole of an fp32
@@ -275,33 +275,141 @@ __device__ __forceinline__ void split_bf16(float x, bf16_t (&o)[TERMS]) {
   }
 }
 
+// lane exchanges without LDS: the pairs (x[l], x[l ^ 16]) and (x[l], x[l ^ 32]) in some order
+__device__ __forceinline__ void swap16(float x, float& a, float& b) {
+  const auto p = __builtin_amdgcn_permlane16_swap(as_u(x), as_u(x), false, false);
+  a = as_f(p[0]);
+  b = as_f(p[1]);
+}
+__device__ __forceinline__ void swap32(float x, float& a, float& b) {
+  const auto p = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
+  a = as_f(p[0]);
+  b = as_f(p[1]);
+}
 // maximum / sum over the four 16-lane groups that hold one query's keys
 __device__ __forceinline__ float across_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+  float a, b;
+  swap16(x, a, b);
+  swap32(fmaxf(a, b), a, b);
+  return fmaxf(a, b);
 }
 __device__ __forceinline__ float across_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+  float a, b;
+  swap16(x, a, b);
+  swap32(a + b, a, b);
+  return a + b;
+}
+// value of lane l ^ 1 / l ^ 2 (quad permutes), l + 4 / l + 8 in a ring of 16 (row rotations)
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return as_f((uint32_t)__builtin_amdgcn_mov_dpp((int)as_u(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
+// maximum / sum over the wave's sixteen quads, each of which holds one value four times
+__device__ __forceinline__ float quads_max(float x) {
+  x = fmaxf(x, dpp<DPP_ROR4>(x));
+  x = fmaxf(x, dpp<DPP_ROR8>(x));
+  return across_max(x);
+}
+__device__ __forceinline__ float quads_sum(float x) {
+  x += dpp<DPP_ROR4>(x);
+  x += dpp<DPP_ROR8>(x);
+  return across_sum(x);
 }
 
+// A query row's own tail, by one wave: running maximum (log2 units), sum, and o[lane] of dim `lane`.  Sixteen tokens at a time, four lanes
+// (16 dims each) to a token; the values of the sixteen are on their way while the scores are made.
+template <typename TQ>
+__device__ __forceinline__ void tail_row(const AttnArgs& a, int b, int n, int hq, int lane, float& m, float& l, float& o) {
+  m = -INFINITY;
+  l = o = 0.f;
+  int T = a.tail_len ? a.tail_len[(int64_t)b * a.tl_bs + (int64_t)n * a.tl_ns] : a.tail_T;
+  T = T < 0 ? 0 : (T > a.tail_T ? a.tail_T : T);
+  const int part = (lane & 3) * 16, tok = lane >> 2, h = hq / a.G;
+  const float to_log2 = a.scale * KV_LOG2E;
+  const TQ* qp = (const TQ*)a.q + (int64_t)b * a.q_bs + (int64_t)n * a.q_ns + (int64_t)hq * a.q_hs + part;
+  const int64_t t_at = (int64_t)b * a.t_bs + (int64_t)n * a.t_ns + (int64_t)h * a.t_hs;
+  const TQ* tk = (const TQ*)a.tk + t_at + part;
+  const TQ* tv = (const TQ*)a.tv + t_at + lane;
+  f32x4 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = Vec4<TQ>::load(qp + i * 4);
+  for (int t0 = 0; t0 < T; t0 += 16) {
+    float x = -INFINITY;
+    if (t0 + tok < T) {
+      f32x4 k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = Vec4<TQ>::load(tk + (int64_t)(t0 + tok) * a.t_ts + i * 4);
+      x = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) x = __builtin_fmaf(q[i][d], k[i][d], x);
+    }
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = t0 + i < T ? (float)tv[(int64_t)(t0 + i) * a.t_ts] : 0.f;
+    x += dpp<DPP_XOR1>(x);                                             // (a quad without a token: -inf throughout)
+    x += dpp<DPP_XOR2>(x);
+    x *= t0 + tok < T ? to_log2 : 1.f;
+    const float mn = fmaxf(m, quads_max(x)), mu = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(x - mu);
+    l = l * f + quads_sum(p);
+    o *= f;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o = __builtin_fmaf(as_f((uint32_t)__builtin_amdgcn_readlane((int)as_u(p), i * 4)), v[i], o);
+  }
+}
+
+// the row's result: one rounding.  Nothing seen: zeros, lse = -inf; a length that is none (the sequence overflowed on the device): NaN
+__device__ __forceinline__ bool no_length(const AttnArgs& a, int len) { return len < 0 || len > a.nblk * KV_BLOCK; }
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * KV_LN2; }
+
 // One workgroup: one (sequence, head), one group of 16 QT query rows, one share of the blocks; its four waves take the blocks in turn,
-// each with its own running maximum / sum / O, and are joined through LDS at the end.
+// each with its own running maximum / sum / O, and are joined through LDS at the end.  With more than one share the results go to the
+// workspace (the rows' tails are one share more, with workgroups of their own); a single share takes the tails in as well and writes
+// the output itself.
 template <typename TQ, int FMT, int QT>
 __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
   constexpr int TQN = sizeof(TQ) == 4 ? 3 : 1;     // bf16 terms of a query element
   constexpr int TP = sizeof(TQ) == 4 ? 3 : 2;      // ... and of a probability
+  constexpr int ROWS = 16 * QT;
   __shared__ __attribute__((aligned(16))) float o_s[4][16][KV_HD + 4];
-  __shared__ float m_s[4][16 * QT], l_s[4][16 * QT];
+  __shared__ __attribute__((aligned(16))) float t_s[ROWS][KV_HD];       // tails
+  __shared__ float m_s[5][ROWS], l_s[5][ROWS];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.nsplit;
-  const int64_t rest = blockIdx.x / a.nsplit;
+  const int split = blockIdx.x % a.nshare;
+  const int64_t rest = blockIdx.x / a.nshare;
   const int rt = (int)(rest % a.row_tiles);
   const int64_t pair = rest / a.row_tiles;
   const int b = (int)(pair / a.H), h = (int)(pair % a.H);
-  const int R = a.N * a.G, row0 = rt * 16 * QT;
+  const int R = a.N * a.G, row0 = rt * ROWS, nrow = min(ROWS, R - row0);
+  const bool direct = a.nshare == 1;
+  if (split == a.nsplit || (direct && a.tk)) {
+    for (int r = wave; r < nrow; r += 4) {
+      const int row = row0 + r;
+      float m, l, o;
+      tail_row<TQ>(a, b, row / a.G, h * a.G + row % a.G, lane, m, l, o);
+      if (direct) {
+        t_s[r][lane] = o;
+        if (lane == 0) {
+          m_s[4][r] = m;
+          l_s[4][r] = l;
+        }
+      } else {
+        const int64_t at = (pair * a.nshare + split) * R + row;
+        a.part_o[at * KV_HD + lane] = o;
+        if (lane == 0) {
+          a.part_ml[at * 2] = m;
+          a.part_ml[at * 2 + 1] = l;
+        }
+      }
+    }
+    if (!direct) return;
+  }
   const int len = a.lens[b];
-  const int blocks = len > 0 ? (min(len, a.nblk * KV_BLOCK) + KV_BLOCK - 1) / KV_BLOCK : 0;
+  const int blocks = no_length(a, len) ? 0 : (len + KV_BLOCK - 1) / KV_BLOCK;
   const int b0 = (int)((int64_t)blocks * split / a.nsplit), b1 = (int)((int64_t)blocks * (split + 1) / a.nsplit);
 
   // queries: B operand, lane (n, g) holds dims g * 16 + step * 8 .. + 7 of row n
@@ -414,7 +522,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
           for (int k = TP - 1; k >= 0; --k) o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d][s], pf[s][k], o[t][d], 0, 0, 0);
     }
   }
-  // ---- join the four waves
+  // ---- join the four waves (and the tails)
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const float ls = across_sum(l[t]);
@@ -427,90 +535,104 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) *(f32x4*)&o_s[wave][n][d * 16 + g * 4] = o[t][d];
     __syncthreads();
-    const int r = tid >> 4, c = (tid & 15) * 4, row = row0 + t * 16 + r;
-    const float m0 = fmaxf(fmaxf(m_s[0][t * 16 + r], m_s[1][t * 16 + r]), fmaxf(m_s[2][t * 16 + r], m_s[3][t * 16 + r]));
+    const int r = tid >> 4, c = (tid & 15) * 4, rr = t * 16 + r, row = row0 + rr;
+    const bool tail = direct && a.tk && rr < nrow;
+    const float mt = tail ? m_s[4][rr] : -INFINITY;
+    const float m0 = fmaxf(fmaxf(fmaxf(m_s[0][rr], m_s[1][rr]), fmaxf(m_s[2][rr], m_s[3][rr])), mt);
     const float ms = m0 == -INFINITY ? 0.f : m0;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
     float ls = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(m_s[w][t * 16 + r] - ms);
+      const float f = __builtin_amdgcn_exp2f(m_s[w][rr] - ms);
       sum += *(const f32x4*)&o_s[w][r][c] * f;
-      ls += l_s[w][t * 16 + r] * f;
+      ls += l_s[w][rr] * f;
+    }
+    if (tail) {
+      const float f = __builtin_amdgcn_exp2f(mt - ms);
+      sum += *(const f32x4*)&t_s[rr][c] * f;
+      ls += l_s[4][rr] * f;
     }
     if (row < R) {
-      const int64_t at = (pair * a.nsplit + split) * R + row;
-      *(f32x4*)(a.part_o + at * KV_HD + c) = sum;
-      if (c == 0) {
-        a.part_ml[at * 2] = m0;
-        a.part_ml[at * 2 + 1] = ls;
+      if (direct) {
+        const float nan = as_f(0x7fc00000u), inv = no_length(a, len) ? nan : (ls == 0.f ? 0.f : 1.f / ls);
+        const int64_t at = ((int64_t)b * a.N + row / a.G) * a.H * a.G + h * a.G + row % a.G;
+        Vec4<TQ>::store((TQ*)a.out + at * KV_HD + c, sum * inv);
+        if (c == 0) a.lse[at] = no_length(a, len) ? nan : lse_of(m0, ls);
+      } else {
+        const int64_t at = (pair * a.nshare + split) * R + row;
+        *(f32x4*)(a.part_o + at * KV_HD + c) = sum;
+        if (c == 0) {
+          a.part_ml[at * 2] = m0;
+          a.part_ml[at * 2 + 1] = ls;
+        }
       }
     }
     __syncthreads();
   }
 }
 
-// One wave per output row: joins the shares of the cache and the row's own tail (operand dtype, scored here in fp32).
-template <typename TQ>
+// Joins the shares of an output row: WPR waves to a row, each with every WPR-th share; lane s weighs share s, then lane d sums dim d.
+template <typename TQ, int WPR>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
-  __shared__ float q_s[4][KV_HD];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  __shared__ float o_s[4][KV_HD], m_s[4], l_s[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sub = wave % WPR;
   const int HQ = a.H * a.G, R = a.N * a.G;
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;           // b, n, query head
   const int64_t rows = (int64_t)a.B * a.N * HQ;
-  const bool there = row < rows;
-  const int64_t rc = there ? row : rows - 1;
+  const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;           // b, n, query head
+  const int64_t rc = row < rows ? row : rows - 1;
   const int hq = (int)(rc % HQ), n = (int)(rc / HQ % a.N), b = (int)(rc / HQ / a.N);
-  const int h = hq / a.G, len = a.lens[b];
-  const int64_t at0 = ((int64_t)b * a.H + h) * a.nsplit * R + n * a.G + hq % a.G;
+  const int64_t at0 = ((int64_t)b * a.H + hq / a.G) * a.nshare * R + n * a.G + hq % a.G;
   float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int s = 0; s < a.nsplit; ++s) {
-    const int64_t at = at0 + (int64_t)s * R;
-    const float ms = a.part_ml[at * 2], ls = a.part_ml[at * 2 + 1], os = a.part_o[at * KV_HD + lane];
-    const float mn = fmaxf(m, ms), mu = mn == -INFINITY ? 0.f : mn;
-    const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(ms - mu);
-    l = l * f0 + ls * f1;
-    o = o * f0 + os * f1;
-    m = mn;
-  }
-  const TQ* qp = (const TQ*)a.q + (int64_t)b * a.q_bs + (int64_t)n * a.q_ns + (int64_t)hq * a.q_hs;
-  q_s[wave][lane] = (float)qp[lane] * (a.scale * KV_LOG2E);
-  __syncthreads();
-  int T = 0;
-  if (a.tk) {
-    T = a.tail_len ? a.tail_len[(int64_t)b * a.tl_bs + (int64_t)n * a.tl_ns] : a.tail_T;
-    T = T < 0 ? 0 : (T > a.tail_T ? a.tail_T : T);
-  }
-  const TQ* tk = (const TQ*)a.tk + (int64_t)b * a.t_bs + (int64_t)n * a.t_ns + (int64_t)h * a.t_hs;
-  const TQ* tv = (const TQ*)a.tv + (int64_t)b * a.t_bs + (int64_t)n * a.t_ns + (int64_t)h * a.t_hs;
-  for (int t0 = 0; t0 < T; t0 += 64) {
-    float x = -INFINITY;
-    if (t0 + lane < T) {
-      x = 0.f;
-#pragma unroll 4
-      for (int d = 0; d < KV_HD; d += 4) {
-        const f32x4 kv = Vec4<TQ>::load(tk + (int64_t)(t0 + lane) * a.t_ts + d);
-        x += kv[0] * q_s[wave][d] + kv[1] * q_s[wave][d + 1] + kv[2] * q_s[wave][d + 2] + kv[3] * q_s[wave][d + 3];
-      }
+  for (int s0 = sub; s0 < a.nshare; s0 += 64 * WPR) {
+    const int s = s0 + lane * WPR;
+    float ms = -INFINITY, ls = 0.f;
+    if (s < a.nshare) {
+      const float2 ml = *(const float2*)(a.part_ml + (at0 + (int64_t)s * R) * 2);
+      ms = ml.x;
+      ls = ml.y;
     }
-    float mx = x;
+    float mx = ms;
 #pragma unroll
     for (int i = 32; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i, 64));
     const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-    const float f0 = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(x - mu);
-    l = l * f0 + wave_sum(p);
-    o *= f0;
+    const float f = __builtin_amdgcn_exp2f(m - mu), w = __builtin_amdgcn_exp2f(ms - mu);
+    l = l * f + wave_sum(ls * w);
+    o *= f;
     m = mn;
-    const int nt = min(64, T - t0);
-    for (int t = 0; t < nt; ++t) o += __shfl(p, t, 64) * (float)tv[(int64_t)(t0 + t) * a.t_ts + lane];
+    const int cnt = min(64, (a.nshare - s0 + WPR - 1) / WPR);
+    const float* po = a.part_o + (at0 + (int64_t)s0 * R) * KV_HD + lane;
+    for (int i0 = 0; i0 < cnt; i0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i0 + i < cnt ? po[(int64_t)(i0 + i) * WPR * R * KV_HD] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o = __builtin_fmaf(as_f((uint32_t)__builtin_amdgcn_readlane((int)as_u(w), (i0 + i) & 63)), v[i], o);
+    }
   }
-  if (there) {
-    // a row that sees nothing: zeros, lse = -inf; a sequence whose length is none (it overflowed on the device): NaN
-    const bool bad = len < 0 || len > a.nblk * KV_BLOCK;
+  if (WPR > 1) {
+    o_s[wave][lane] = o;
+    if (lane == 0) {
+      m_s[wave] = m;
+      l_s[wave] = l;
+    }
+    __syncthreads();
+    m = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
+    const float mu = m == -INFINITY ? 0.f : m;
+    o = l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(m_s[w] - mu);
+      o += o_s[w][lane] * f;
+      l += l_s[w] * f;
+    }
+    if (sub) return;
+  }
+  if (row < rows) {
+    const bool bad = no_length(a, a.lens[b]);
     const float nan = as_f(0x7fc00000u);
-    const float res = bad ? nan : (l == 0.f ? 0.f : o / l);
-    ((TQ*)a.out)[row * KV_HD + lane] = (TQ)res;
-    if (lane == 0) a.lse[row] = bad ? nan : (l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * KV_LN2);
+    ((TQ*)a.out)[row * KV_HD + lane] = (TQ)(bad ? nan : (l == 0.f ? 0.f : o / l));
+    if (lane == 0) a.lse[row] = bad ? nan : lse_of(m, l);
   }
 }
 
@@ -518,6 +640,13 @@ template <typename TQ, int FMT>
 void launch_attn(const AttnArgs& a, int qt, unsigned grid, hipStream_t st) {
   if (qt == 1) hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 1>), dim3(grid), dim3(256), 0, st, a);
   else hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 2>), dim3(grid), dim3(256), 0, st, a);
+}
+
+template <typename TQ>
+void launch_join(const AttnArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.B * a.N * a.H * a.G;
+  if (a.nshare > 16) hipLaunchKernelGGL((kv8_attn_join_kernel<TQ, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv8_attn_join_kernel<TQ, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
 }
 
 bool kv8_bad_fmt(int fmt) { return fmt != FMT_INT8 && fmt != FMT_E4M3; }
@@ -595,7 +724,7 @@ extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens) {
 }
 
 extern "C" int64_t t2s_kv8_attn_workspace_bytes(int B, int N, int H, int G, int splits) {
-  return (int64_t)B * H * splits * N * G * (KV_HD + 2) * 4;
+  return splits > 1 ? (int64_t)B * H * (splits + 1) * N * G * (KV_HD + 2) * 4 : 0;
 }
 
 extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride, const void* k8, const void* v8,
@@ -604,7 +733,7 @@ extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row
                             const int32_t* tail_len, int64_t tl_batch_stride, int64_t tl_row_stride, int tail_T, void* out, float* lse,
                             void* workspace, int64_t workspace_bytes, int splits, int B, int N, int H, int G, int nblk, float scale, int dtype,
                             int fmt, t2s_stream_t stream) {
-  T2S_CHECK_ARG(q && k8 && v8 && k_scale && v_scale && lens && out && lse && workspace, "kv8_attn: null pointer");
+  T2S_CHECK_ARG(q && k8 && v8 && k_scale && v_scale && lens && out && lse && (workspace || splits == 1), "kv8_attn: null pointer");
   T2S_CHECK_ARG(B > 0 && N > 0 && H > 0 && G > 0 && nblk > 0 && nblk < (1 << 25) && (int64_t)N * G < (1 << 24) && (int64_t)B * H < (1 << 24),
                 "kv8_attn: bad shape B=%d N=%d H=%d G=%d nblk=%d", B, N, H, G, nblk);
   T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "kv8_attn: bad dtype %d", dtype);
@@ -624,23 +753,24 @@ extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   a.tk = tail_T > 0 ? tail_k : nullptr; a.tv = tail_v; a.t_bs = t_batch_stride; a.t_ns = t_row_stride; a.t_ts = t_token_stride; a.t_hs = t_head_stride;
   a.tail_len = tail_len; a.tl_bs = tl_batch_stride; a.tl_ns = tl_row_stride; a.tail_T = tail_T;
   a.out = out; a.lse = lse;
+  a.scale = scale; a.B = B; a.N = N; a.H = H; a.G = G; a.nblk = nblk; a.nsplit = splits; a.nshare = splits > 1 && a.tk ? splits + 1 : splits;
+  a.row_tiles = (rows + 16 * qt - 1) / (16 * qt);
   a.part_o = (float*)workspace;
-  a.part_ml = a.part_o + (int64_t)B * H * splits * rows * KV_HD;
-  a.scale = scale; a.B = B; a.N = N; a.H = H; a.G = G; a.nblk = nblk; a.nsplit = splits; a.row_tiles = (rows + 16 * qt - 1) / (16 * qt);
-  const int64_t grid = (int64_t)B * H * a.row_tiles * splits, join = ((int64_t)B * N * H * G + 3) / 4;
-  T2S_CHECK_ARG(grid < ((int64_t)1 << 31) && join < ((int64_t)1 << 31), "kv8_attn: too many workgroups");
+  a.part_ml = a.part_o + (int64_t)B * H * a.nshare * rows * KV_HD;
+  const int64_t grid = (int64_t)B * H * a.row_tiles * a.nshare;
+  T2S_CHECK_ARG(grid < ((int64_t)1 << 31) && (int64_t)B * H * rows < ((int64_t)1 << 31), "kv8_attn: too many workgroups");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == T2S_BF16) {
     if (fmt == FMT_INT8) launch_attn<bf16_t, FMT_INT8>(a, qt, (unsigned)grid, st);
     else launch_attn<bf16_t, FMT_E4M3>(a, qt, (unsigned)grid, st);
-    T2S_CHECK_LAUNCH("kv8_attn");
-    hipLaunchKernelGGL(kv8_attn_join_kernel<bf16_t>, dim3((unsigned)join), dim3(256), 0, st, a);
   } else {
     if (fmt == FMT_INT8) launch_attn<float, FMT_INT8>(a, qt, (unsigned)grid, st);
     else launch_attn<float, FMT_E4M3>(a, qt, (unsigned)grid, st);
-    T2S_CHECK_LAUNCH("kv8_attn");
-    hipLaunchKernelGGL(kv8_attn_join_kernel<float>, dim3((unsigned)join), dim3(256), 0, st, a);
   }
+  T2S_CHECK_LAUNCH("kv8_attn");
+  if (a.nshare == 1) return 0;
+  if (dtype == T2S_BF16) launch_join<bf16_t>(a, st);
+  else launch_join<float>(a, st);
   T2S_CHECK_LAUNCH("kv8_attn_join");
   return 0;
 }

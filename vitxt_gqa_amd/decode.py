@@ -222,9 +222,9 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
     if N == 0:
         return out, lse
     splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len)
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device)
+    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
     X.check(_launch(cache._index, X.lib().t2s_kv8_attn, q.data_ptr(), sq[0], sq[1], sq[2], *cache._ptrs, tk, tv, st[0], st[1], st[2], st[3], tl, tls[0], tls[1], T,
-                    out.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, _DTYPES[q.dtype][0], cache._fmt), "t2s_kv8_attn")
+                    out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, _DTYPES[q.dtype][0], cache._fmt), "t2s_kv8_attn")
     return out, lse
 
 
