@@ -381,7 +381,7 @@ int t2s_gemm_wgrad(const void* dy, const void* x, float* dw, float* slabs, int64
  *   (NULL: tail_T) of the row's own tail_T tail tokens (tail_k / tail_v in dtype, element (b, n, t, h, d) by their strides; NULL: none);
  *   lse: natural log-sum-exp [B, N, H G].  A row that sees nothing: out 0, lse -inf.  splits: shares of the token axis
  *   (t2s_kv8_attn_splits for about max_tokens tokens; any positive number is right for any length); workspace as
- *   t2s_kv8_attn_workspace_bytes says (0 bytes for a single share: it may be NULL), contents on entry irrelevant. */
+ *   t2s_kv8_attn_workspace_bytes says (NULL where that is 0 bytes), contents on entry irrelevant. */
 #define T2S_KV_INT8 0
 #define T2S_KV_E4M3 1
 int t2s_kv8_append(const void* k, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, const void* v,
@@ -390,7 +390,7 @@ int t2s_kv8_append(const void* k, int64_t k_batch_stride, int64_t k_row_stride, 
                    int B, int H, int T, int L, int nblk, int dtype, int fmt, t2s_stream_t stream);
 int t2s_kv8_dequantize(const void* k8, const void* v8, const float* k_scale, const float* v_scale, const int32_t* lens, void* k, void* v,
                        int B, int H, int nblk, int dtype, int fmt, t2s_stream_t stream);
-int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens);
+int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens, int dtype);
 int64_t t2s_kv8_attn_workspace_bytes(int B, int N, int H, int G, int splits);
 int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride, const void* k8, const void* v8,
                  const float* k_scale, const float* v_scale, const int32_t* lens, const void* tail_k, const void* tail_v,

@@ -127,7 +127,7 @@ def test_c_abi_refuses(lib):
         assert lib.t2s_beam_select(*a) != 0 and text in lib.t2s_last_error(), (i, lib.t2s_last_error())
     assert lib.t2s_beam_reorder(p, p, 1, 1, 33, 16, 16, None) != 0 and b"bad shape" in lib.t2s_last_error()
     assert lib.t2s_beam_reorder(p, p, 1, 1, 3, 16, 32, None) != 0 and b"bytes" in lib.t2s_last_error()
-    assert lib.t2s_kv8_attn_splits(0, 1, 1, 1, 64) == 0 and lib.t2s_kv8_attn_splits(1, 1, 1, 1, 0) == 1
+    assert lib.t2s_kv8_attn_splits(0, 1, 1, 1, 64, 0) == 0 and lib.t2s_kv8_attn_splits(1, 1, 1, 1, 0, 1) == 1
     assert lib.t2s_beam_select_workspace_bytes(0, 1, 1, 1) == 0
 
 

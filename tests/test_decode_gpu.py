@@ -4,7 +4,8 @@ Tolerances, u = 2^-24 (half an fp32 step), w = 2^-8 (half a bf16 step):
   append        none: codes and scales are defined by exact products
   attend        a score is 64 products (each exact: <= 8 x 8 significant bits; three terms of an fp32 query) summed in fp32 by the matrix pipe, then two
                 rescalings: |d score| <= 200 u S, S = scale * max sum |q_d k_d|.  out: 2 |d score| vmax from the weights, the sums over tokens and shares
-                (L / 32 + 64) u vmax, probabilities held in 16 bits (bf16: w^2 vmax) or 24 (fp32: u vmax), one rounding of the result (bf16: w |out|).
+                (L / 32 + 64) u vmax, probabilities held in f16 (bf16 results: off by 2^-12 of themselves, or where they are subnormal by 2^-25 of
+                the largest, so by (2^-12 + L 2^-25) vmax over a row) or in 24 bits (fp32: u vmax), one rounding of the result (bf16: w |out|).
                 lse: |d score| + (L / 32 + 64) u + u |lse|
   beam_select   the order is the 64-bit statement's wherever neighbours differ by more than the tolerance (and where they are equal); a score's
                 error is that of log sum exp: terms e^d with d rounded in fp32 (104 u at most before they vanish) and summed: 160 u, + u |score|
@@ -46,7 +47,7 @@ def _check_attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125
     ref, rlse, S, vmax = attend_ref(q, read_cache(cache), tail_k, tail_v, tail_len, scale)
     L = cache.capacity
     ds = 200 * U * S
-    terms = (W * W if q.dtype == torch.bfloat16 else U) + (L / 32 + 64) * U
+    terms = (2.0 ** -12 + L * 2.0 ** -25 if q.dtype == torch.bfloat16 else U) + (L / 32 + 64) * U
     tol = (2 * ds + terms) * vmax + (W if q.dtype == torch.bfloat16 else U) * ref.abs() + 1e-30
     err = (out.cpu().double() - ref).abs()
     assert out.dtype == q.dtype and bool((err <= tol).all()), "out off by %.3g of %.3g" % (err.max(), tol.max())

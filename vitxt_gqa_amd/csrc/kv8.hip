@@ -20,6 +20,9 @@
 // shuffles between the two products, and every load of the pass is 16 contiguous bytes per lane.
 #include "common.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 constexpr int KV_BLOCK = 64;                       // tokens per block
@@ -83,6 +86,25 @@ __device__ __forceinline__ bf16x8 decode8(uint32_t lo, uint32_t hi) {
   const b2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
   const b2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+
+// ... and the f16 operand (exact: eleven significant bits, e4m3's 2^-9 .. 448 within f16's range)
+template <int FMT>
+__device__ __forceinline__ f16x8 decode8_f16(uint32_t lo, uint32_t hi) {
+  typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+  if (FMT == FMT_INT8) {
+    // code + 128 as the low byte of an f16 is 1024 + 128 + code: two bytes a v_perm_b32, two subtractions an instruction
+    const h2 off = {(_Float16)1152.f, (_Float16)1152.f};
+    const uint32_t l = lo ^ 0x80808080u, h = hi ^ 0x80808080u;
+    const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, l, 0x04010400u)) - off, b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, l, 0x04030402u)) - off;
+    const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, h, 0x04010400u)) - off, d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, h, 0x04030402u)) - off;
+    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+  const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // word position of token group tg (tokens 4 tg .. 4 tg + 3) inside a value row: p / 4 of the order above
@@ -262,7 +284,8 @@ struct AttnArgs {
   float* part_o;        // [B * H][nshare][R][64]
   float* part_ml;       // [B * H][nshare][R][2]: running maximum (log2 units), sum
   float scale;
-  int B, N, H, G, nblk, nsplit, nshare, row_tiles;      // nshare: nsplit shares of the cache, and one more for the tails where nsplit > 1
+  int B, N, H, G, nblk, row_tiles;
+  int nsplit, nshare, tail_groups;      // shares of the cache; one more for the tails unless a single share does it all; workgroups for the tails
 };
 
 // x as a sum of TERMS bf16 numbers (8 significant bits each): 1 for what is bf16 already, 2 keep 16 bits, 3 the whole of an fp32
@@ -317,6 +340,43 @@ __device__ __forceinline__ float quads_sum(float x) {
   return across_sum(x);
 }
 
+// The second product of a block: V^T P^T, codes times probabilities, for the tokens of step s of a lane.  A bf16 result takes its
+// probabilities as f16: eleven bits, off by 2^-12 at most (and by 2^-25 of the largest where they are that small) before the result
+// is rounded to eight bits.  An fp32 result takes them as three bf16 terms, which are all of an fp32 number.
+template <typename TQ, int FMT>
+struct Second;
+template <int FMT>
+struct Second<bf16_t, FMT> {
+  typedef f16x8 V;
+  struct P { f16x8 s[2]; };
+  static __device__ __forceinline__ V decode(uint32_t lo, uint32_t hi) { return decode8_f16<FMT>(lo, hi); }
+  static __device__ __forceinline__ void put(P& p, int i, int r, float x) { p.s[i >> 1][(i & 1) * 4 + r] = (_Float16)x; }
+  static __device__ __forceinline__ f32x4 mul(const V (&v)[2], const P& p) {
+    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1], p.s[1], __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0], p.s[0], z, 0, 0, 0), 0, 0, 0);
+  }
+};
+template <int FMT>
+struct Second<float, FMT> {
+  typedef bf16x8 V;
+  struct P { bf16x8 s[2][3]; };
+  static __device__ __forceinline__ V decode(uint32_t lo, uint32_t hi) { return decode8<FMT>(lo, hi); }
+  static __device__ __forceinline__ void put(P& p, int i, int r, float x) {
+    bf16_t w[3];
+    split_bf16<3>(x, w);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) p.s[i >> 1][k][(i & 1) * 4 + r] = w[k];
+  }
+  static __device__ __forceinline__ f32x4 mul(const V (&v)[2], const P& p) {
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[s], p.s[s][k], z, 0, 0, 0);
+    return z;
+  }
+};
+
 // A query row's own tail, by one wave: running maximum (log2 units), sum, and o[lane] of dim `lane`.  Sixteen tokens at a time, four lanes
 // (16 dims each) to a token; the values of the sixteen are on their way while the scores are made.
 template <typename TQ>
@@ -334,24 +394,26 @@ __device__ __forceinline__ void tail_row(const AttnArgs& a, int b, int n, int hq
   f32x4 q[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) q[i] = Vec4<TQ>::load(qp + i * 4);
-  for (int t0 = 0; t0 < T; t0 += 16) {
-    float x = -INFINITY;
-    if (t0 + tok < T) {
+  // (whole sixteens of the tail's capacity are requested before the row's own length is there; what is behind the length is not used)
+  for (int t0 = 0; t0 < a.tail_T; t0 += 16) {
+    if (t0 > 0 && t0 >= T) break;
+    float x = 0.f, v[16];
+    if (t0 + tok < a.tail_T) {
       f32x4 k[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) k[i] = Vec4<TQ>::load(tk + (int64_t)(t0 + tok) * a.t_ts + i * 4);
-      x = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int d = 0; d < 4; ++d) x = __builtin_fmaf(q[i][d], k[i][d], x);
     }
-    float v[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = t0 + i < T ? (float)tv[(int64_t)(t0 + i) * a.t_ts] : 0.f;
-    x += dpp<DPP_XOR1>(x);                                             // (a quad without a token: -inf throughout)
+    for (int i = 0; i < 16; ++i) v[i] = (float)tv[(int64_t)min(t0 + i, a.tail_T - 1) * a.t_ts];
+    x += dpp<DPP_XOR1>(x);
     x += dpp<DPP_XOR2>(x);
-    x *= t0 + tok < T ? to_log2 : 1.f;
+    x = t0 + tok < T ? x * to_log2 : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = t0 + i < T ? v[i] : 0.f;
     const float mn = fmaxf(m, quads_max(x)), mu = mn == -INFINITY ? 0.f : mn;
     const float f = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(x - mu);
     l = l * f + quads_sum(p);
@@ -368,26 +430,24 @@ __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -I
 
 // One workgroup: one (sequence, head), one group of 16 QT query rows, one share of the blocks; its four waves take the blocks in turn,
 // each with its own running maximum / sum / O, and are joined through LDS at the end.  With more than one share the results go to the
-// workspace (the rows' tails are one share more, with workgroups of their own); a single share takes the tails in as well and writes
-// the output itself.
+// workspace (the rows' tails are one share more, with workgroups of their own); a single share takes the tails of a few rows in as well and
+// writes the output itself.
 template <typename TQ, int FMT, int QT>
-__global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void kv8_attn_kernel(AttnArgs a) {
+  typedef Second<TQ, FMT> PV;
   constexpr int TQN = sizeof(TQ) == 4 ? 3 : 1;     // bf16 terms of a query element
-  constexpr int TP = sizeof(TQ) == 4 ? 3 : 2;      // ... and of a probability
   constexpr int ROWS = 16 * QT;
   __shared__ __attribute__((aligned(16))) float o_s[4][16][KV_HD + 4];
   __shared__ __attribute__((aligned(16))) float t_s[ROWS][KV_HD];       // tails
   __shared__ float m_s[5][ROWS], l_s[5][ROWS];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.nshare;
-  const int64_t rest = blockIdx.x / a.nshare;
-  const int rt = (int)(rest % a.row_tiles);
-  const int64_t pair = rest / a.row_tiles;
-  const int b = (int)(pair / a.H), h = (int)(pair % a.H);
-  const int R = a.N * a.G, row0 = rt * ROWS, nrow = min(ROWS, R - row0);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int pair = blockIdx.x, b = pair / a.H, h = pair - b * a.H;
+  const int R = a.N * a.G, row0 = blockIdx.y * ROWS, nrow = min(ROWS, R - row0);
   const bool direct = a.nshare == 1;
-  if (split == a.nsplit || (direct && a.tk)) {
-    for (int r = wave; r < nrow; r += 4) {
+  // (the tails go first: their workgroups, a row to a wave, are short and end long before the others)
+  const int split = (int)blockIdx.z - a.tail_groups, share = split < 0 ? a.nsplit : split;
+  if (split < 0 || (direct && a.tk)) {
+    for (int r = direct ? wave : (int)blockIdx.z * 4 + wave; r < nrow; r += direct ? 4 : ROWS) {
       const int row = row0 + r;
       float m, l, o;
       tail_row<TQ>(a, b, row / a.G, h * a.G + row % a.G, lane, m, l, o);
@@ -398,7 +458,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
           l_s[4][r] = l;
         }
       } else {
-        const int64_t at = (pair * a.nshare + split) * R + row;
+        const int64_t at = ((int64_t)pair * a.nshare + share) * R + row;
         a.part_o[at * KV_HD + lane] = o;
         if (lane == 0) {
           a.part_ml[at * 2] = m;
@@ -410,9 +470,11 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
   }
   const int len = a.lens[b];
   const int blocks = no_length(a, len) ? 0 : (len + KV_BLOCK - 1) / KV_BLOCK;
-  const int b0 = (int)((int64_t)blocks * split / a.nsplit), b1 = (int)((int64_t)blocks * (split + 1) / a.nsplit);
+  const int per = blocks / a.nsplit, over = blocks - per * a.nsplit;
+  const int b0 = split * per + min(split, over), b1 = b0 + per + (split < over ? 1 : 0);
 
-  // queries: B operand, lane (n, g) holds dims g * 16 + step * 8 .. + 7 of row n
+  // queries: B operand, lane (n, g) holds dims g * 16 + step * 8 .. + 7 of row n.  A negative scale's sign goes into them.
+  const float to_log2 = fabsf(a.scale) * KV_LOG2E;
   bf16x8 qf[QT][2][TQN];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -427,7 +489,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           bf16_t w[TQN];
-          split_bf16<TQN>(f[i], w);
+          split_bf16<TQN>(a.scale < 0.f ? -f[i] : f[i], w);
 #pragma unroll
           for (int k = 0; k < TQN; ++k) qf[t][s][k][e * 4 + i] = w[k];
         }
@@ -442,19 +504,91 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float to_log2 = a.scale * KV_LOG2E;
-  const int64_t base = pair * a.nblk;
-  for (int blk = b0 + wave; blk < b1; blk += 4) {
+  const int64_t base = (int64_t)pair * a.nblk;
+  // A block's keys are requested while the block before them is worked on (8 sequences x 12 heads x 5 rows over 10 120 tokens 15.2 us, 16.1 without;
+  // 64 x 3 heads x 80 rows 90 us, 106), its values at the head of its own step: their turn comes behind the scores.
+  uint4 kr[4];
+  float ks_next = 0.f, vs_next = 0.f;
+  auto fetch_k = [&](const int blk) {
     const uint8_t* kp = a.k8 + (base + blk) * KV_BYTES + n * KV_HD + g * 16;
-    const uint8_t* vp = a.v8 + (base + blk) * KV_BYTES + n * KV_BLOCK + g * 16;
-    const float ks = a.ks[base + blk] * to_log2, vs = a.vs[base + blk];
-    uint4 kr[4], vr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) kr[i] = *(const uint4*)(kp + i * 16 * KV_HD);
+    ks_next = a.ks[base + blk];
+    vs_next = a.vs[base + blk];
+  };
+  // one block; `whole`: all of its tokens are there (only the last block of a sequence is masked, by code of its own)
+  auto step = [&](const int blk, auto whole) {
+    constexpr bool last = !decltype(whole)::value;
+    const uint8_t* vp = a.v8 + (base + blk) * KV_BYTES + n * KV_BLOCK + g * 16;
+    const float ks = ks_next * to_log2, vs = vs_next;
+    uint4 vr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) vr[i] = *(const uint4*)(vp + i * 16 * KV_BLOCK);
     const int left = len - blk * KV_BLOCK;                  // tokens of the block that are there
-    if (left < KV_BLOCK) {                                  // codes behind the length count as zeros (an e4m3 NaN there would outlive p = 0)
+    bf16x8 kf[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kf[i][0] = decode8<FMT>(kr[i].x, kr[i].y);
+      kf[i][1] = decode8<FMT>(kr[i].z, kr[i].w);
+    }
+    if (blk + 4 < b1) fetch_k(blk + 4);
+    // scores of all row tiles, then one look at their maxima, then the probabilities: independent work side by side in each phase
+    f32x4 x[QT][4];
+    float mx[QT];
+    bool moves = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int k = TQN - 1; k >= 0; --k) x[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][s], qf[t][s][k], x[t][i], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      mx[t] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (last) x[t][i][r] = i * 16 + g * 4 + r < left ? x[t][i][r] : -INFINITY;
+          mx[t] = fmaxf(mx[t], x[t][i][r]);
+        }
+      mx[t] = across_max(mx[t]) * ks;
+      moves |= mx[t] > m[t] + 8.f;
+    }
+    // the maximum need not be exact: it moves only when a score exceeds it by 2^8 (probabilities then stay below 2^8: in range, and as
+    // precise as below 1), which after the first block hardly happens
+    if (__any(moves)) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const float mn = fmaxf(m[t], mx[t]);
+        const float f = m[t] == mn ? 1.f : __builtin_amdgcn_exp2f(m[t] - mn);      // (0 the first time: exp2(-inf))
+        m[t] = mn;
+        l[t] *= f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[t][d] *= f;
+      }
+    }
+    typename PV::P pf[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float ms = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float e = __builtin_fmaf(x[t][i][r], ks, -ms);
+          if (last) e = i * 16 + g * 4 + r < left ? e : -INFINITY;                 // (-inf times a scale of 0)
+          const float p = __builtin_amdgcn_exp2f(e);
+          l[t] += p;
+          PV::put(pf[t], i, r, p);
+        }
+    }
+    if (last) {                                             // codes behind the length count as zeros (an e4m3 NaN there would outlive p = 0)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t* w = (uint32_t*)&vr[i];
@@ -465,63 +599,23 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
         }
       }
     }
-    bf16x8 kf[4][2], vf[4][2];
+    // values: a tile of 16 dims at a time, codes times probabilities, then the block's scale
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      kf[i][0] = decode8<FMT>(kr[i].x, kr[i].y);
-      kf[i][1] = decode8<FMT>(kr[i].z, kr[i].w);
-    }
+    for (int d = 0; d < 4; ++d) {
+      const typename PV::V vf[2] = {PV::decode(vr[d].x, vr[d].y), PV::decode(vr[d].z, vr[d].w)};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      vf[i][0] = decode8<FMT>(vr[i].x, vr[i].y);
-      vf[i][1] = decode8<FMT>(vr[i].z, vr[i].w);
-    }
+      for (int t = 0; t < QT; ++t) {
+        const f32x4 z = PV::mul(vf, pf[t]);
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float x[4][4];
-      float mx = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int k = TQN - 1; k >= 0; --k) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][s], qf[t][s][k], acc, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[i][r] = i * 16 + g * 4 + r < left ? acc[r] * ks : -INFINITY;
-          mx = fmaxf(mx, x[i][r]);
-        }
+        for (int r = 0; r < 4; ++r) o[t][d][r] = __builtin_fmaf(z[r], vs, o[t][d][r]);
       }
-      mx = across_max(mx);
-      if (mx > m[t]) {
-        const float f = __builtin_amdgcn_exp2f(m[t] - mx);            // (0 the first time: exp2(-inf))
-        m[t] = mx;
-        l[t] *= f;
-#pragma unroll
-        for (int d = 0; d < 4; ++d) o[t][d] *= f;
-      }
-      const float ms = m[t] == -INFINITY ? 0.f : m[t];
-      bf16x8 pf[2][TP];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float p = __builtin_amdgcn_exp2f(x[i][r] - ms);
-          l[t] += p;
-          bf16_t w[TP];
-          split_bf16<TP>(p * vs, w);
-#pragma unroll
-          for (int k = 0; k < TP; ++k) pf[i >> 1][k][(i & 1) * 4 + r] = w[k];
-        }
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int k = TP - 1; k >= 0; --k) o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[d][s], pf[s][k], o[t][d], 0, 0, 0);
     }
-  }
+  };
+  const int whole1 = min(b1, len / KV_BLOCK);               // (b1 <= blocks: at most one block behind it)
+  int blk = b0 + wave;
+  if (blk < b1) fetch_k(blk);
+  for (; blk < whole1; blk += 4) step(blk, std::true_type{});
+  if (blk < b1) step(blk, std::false_type{});
   // ---- join the four waves (and the tails)
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -560,7 +654,7 @@ __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
         Vec4<TQ>::store((TQ*)a.out + at * KV_HD + c, sum * inv);
         if (c == 0) a.lse[at] = no_length(a, len) ? nan : lse_of(m0, ls);
       } else {
-        const int64_t at = (pair * a.nshare + split) * R + row;
+        const int64_t at = ((int64_t)pair * a.nshare + share) * R + row;
         *(f32x4*)(a.part_o + at * KV_HD + c) = sum;
         if (c == 0) {
           a.part_ml[at * 2] = m0;
@@ -637,9 +731,14 @@ __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
 }
 
 template <typename TQ, int FMT>
-void launch_attn(const AttnArgs& a, int qt, unsigned grid, hipStream_t st) {
-  if (qt == 1) hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 1>), dim3(grid), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 2>), dim3(grid), dim3(256), 0, st, a);
+void launch_attn(const AttnArgs& a, int qt, hipStream_t st) {
+  const dim3 grid((unsigned)(a.B * a.H), (unsigned)a.row_tiles, (unsigned)(a.nsplit + a.tail_groups));
+  if (qt == 1) hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 1>), grid, dim3(256), 0, st, a);
+  else if (qt == 2) hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 2>), grid, dim3(256), 0, st, a);
+  else if constexpr (sizeof(TQ) == 2) {
+    if (qt == 3) hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 3>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv8_attn_kernel<TQ, FMT, 4>), grid, dim3(256), 0, st, a);
+  }
 }
 
 template <typename TQ>
@@ -649,10 +748,19 @@ void launch_join(const AttnArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL((kv8_attn_join_kernel<TQ, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
 }
 
+// rows of a (sequence, head) whose tails a single share still takes in: four waves, two rows each (12 rows over 600 tokens and a tail
+// of 12, 16 sequences: 17.1 us in one launch, 14.3 with workgroups for the tails and a join; 5 rows: 12.9 and 14.1)
+constexpr int DIRECT_ROWS = 8;
+
 bool kv8_bad_fmt(int fmt) { return fmt != FMT_INT8 && fmt != FMT_E4M3; }
 
-// query tiles (of 16 rows) per workgroup
-int attn_row_tiles(int rows) { return rows > 16 ? 2 : 1; }
+// Row groups of a (sequence, head), each of which reads its cache: as few as registers allow (64 rows; fp32, with three terms to everything,
+// 32), of equal size; returns the 16-row tiles of a group.
+int attn_row_tiles(int rows, int dtype, int* groups) {
+  const int most = dtype == T2S_BF16 ? 64 : 32;
+  *groups = (rows + most - 1) / most;
+  return ((rows + *groups - 1) / *groups + 15) / 16;
+}
 
 }  // namespace
 
@@ -712,19 +820,21 @@ extern "C" int t2s_kv8_dequantize(const void* k8, const void* v8, const float* k
   return 0;
 }
 
-extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens) {
+extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens, int dtype) {
   if (B <= 0 || N <= 0 || H <= 0 || G <= 0) return 0;
   const int blocks = max_tokens > 0 ? (max_tokens + KV_BLOCK - 1) / KV_BLOCK : 1;
-  const int rows = N * G, qt = attn_row_tiles(rows);
-  const int64_t pairs = (int64_t)B * H * ((rows + 16 * qt - 1) / (16 * qt));
-  int64_t s = (2048 + pairs - 1) / pairs;
-  const int64_t most = (blocks + 7) / 8;          // two blocks at least for each wave of a share
-  if (s > most) s = most;
+  int groups;
+  attn_row_tiles(N * G, dtype, &groups);
+  const int64_t pairs = (int64_t)B * H * groups;
+  // Few pairs: as many shares as three workgroups to a CU, of 8 blocks (two to a wave) at least.  Many pairs: shares of 20 blocks, so that
+  // short sequences leave no long ones to wait for.  Measured, us (5 rows, 10 120 tokens): 12 pairs 1 share 37, 20 shares 9.9, 64 13.7; 96 pairs
+  // 1 share 37, 8 15.2, 32 17.7; 768 pairs of ragged lengths 1 share 113, 8 103, 32 120.
+  const int64_t s = 768 / pairs >= 2 ? std::min((int64_t)768 / pairs, (int64_t)(blocks + 7) / 8) : (int64_t)(blocks + 19) / 20;
   return (int)(s < 1 ? 1 : s);
 }
 
 extern "C" int64_t t2s_kv8_attn_workspace_bytes(int B, int N, int H, int G, int splits) {
-  return splits > 1 ? (int64_t)B * H * (splits + 1) * N * G * (KV_HD + 2) * 4 : 0;
+  return splits > 1 || N * G > DIRECT_ROWS ? (int64_t)B * H * (splits + 1) * N * G * (KV_HD + 2) * 4 : 0;
 }
 
 extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, int64_t q_head_stride, const void* k8, const void* v8,
@@ -733,7 +843,7 @@ extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row
                             const int32_t* tail_len, int64_t tl_batch_stride, int64_t tl_row_stride, int tail_T, void* out, float* lse,
                             void* workspace, int64_t workspace_bytes, int splits, int B, int N, int H, int G, int nblk, float scale, int dtype,
                             int fmt, t2s_stream_t stream) {
-  T2S_CHECK_ARG(q && k8 && v8 && k_scale && v_scale && lens && out && lse && (workspace || splits == 1), "kv8_attn: null pointer");
+  T2S_CHECK_ARG(q && k8 && v8 && k_scale && v_scale && lens && out && lse && (workspace || !workspace_bytes), "kv8_attn: null pointer");
   T2S_CHECK_ARG(B > 0 && N > 0 && H > 0 && G > 0 && nblk > 0 && nblk < (1 << 25) && (int64_t)N * G < (1 << 24) && (int64_t)B * H < (1 << 24),
                 "kv8_attn: bad shape B=%d N=%d H=%d G=%d nblk=%d", B, N, H, G, nblk);
   T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "kv8_attn: bad dtype %d", dtype);
@@ -746,26 +856,27 @@ extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   T2S_CHECK_ARG((uintptr_t)k8 % 16 == 0 && (uintptr_t)v8 % 16 == 0 && (uintptr_t)workspace % 16 == 0, "kv8_attn: cache and workspace must be aligned to 16 bytes");
   T2S_CHECK_ARG(splits >= 1 && workspace_bytes >= t2s_kv8_attn_workspace_bytes(B, N, H, G, splits), "kv8_attn: workspace of %lld bytes is too small for %d shares",
                 (long long)workspace_bytes, splits);
-  const int rows = N * G, qt = attn_row_tiles(rows);
+  int groups;
+  const int rows = N * G, qt = attn_row_tiles(rows, dtype, &groups);
   AttnArgs a;
   a.q = q; a.q_bs = q_batch_stride; a.q_ns = q_row_stride; a.q_hs = q_head_stride;
   a.k8 = (const uint8_t*)k8; a.v8 = (const uint8_t*)v8; a.ks = k_scale; a.vs = v_scale; a.lens = lens;
   a.tk = tail_T > 0 ? tail_k : nullptr; a.tv = tail_v; a.t_bs = t_batch_stride; a.t_ns = t_row_stride; a.t_ts = t_token_stride; a.t_hs = t_head_stride;
   a.tail_len = tail_len; a.tl_bs = tl_batch_stride; a.tl_ns = tl_row_stride; a.tail_T = tail_T;
   a.out = out; a.lse = lse;
-  a.scale = scale; a.B = B; a.N = N; a.H = H; a.G = G; a.nblk = nblk; a.nsplit = splits; a.nshare = splits > 1 && a.tk ? splits + 1 : splits;
-  a.row_tiles = (rows + 16 * qt - 1) / (16 * qt);
+  a.scale = scale; a.B = B; a.N = N; a.H = H; a.G = G; a.nblk = nblk; a.nsplit = splits; a.nshare = a.tk && (splits > 1 || rows > DIRECT_ROWS) ? splits + 1 : splits;
+  a.tail_groups = a.nshare > splits ? (std::min(rows, 16 * qt) + 3) / 4 : 0;
+  a.row_tiles = groups;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + (int64_t)B * H * a.nshare * rows * KV_HD;
-  const int64_t grid = (int64_t)B * H * a.row_tiles * a.nshare;
-  T2S_CHECK_ARG(grid < ((int64_t)1 << 31) && (int64_t)B * H * rows < ((int64_t)1 << 31), "kv8_attn: too many workgroups");
+  T2S_CHECK_ARG(a.row_tiles <= 65535 && splits <= 65000 && (int64_t)B * H * rows < ((int64_t)1 << 31), "kv8_attn: too many rows or shares");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == T2S_BF16) {
-    if (fmt == FMT_INT8) launch_attn<bf16_t, FMT_INT8>(a, qt, (unsigned)grid, st);
-    else launch_attn<bf16_t, FMT_E4M3>(a, qt, (unsigned)grid, st);
+    if (fmt == FMT_INT8) launch_attn<bf16_t, FMT_INT8>(a, qt, st);
+    else launch_attn<bf16_t, FMT_E4M3>(a, qt, st);
   } else {
-    if (fmt == FMT_INT8) launch_attn<float, FMT_INT8>(a, qt, (unsigned)grid, st);
-    else launch_attn<float, FMT_E4M3>(a, qt, (unsigned)grid, st);
+    if (fmt == FMT_INT8) launch_attn<float, FMT_INT8>(a, qt, st);
+    else launch_attn<float, FMT_E4M3>(a, qt, st);
   }
   T2S_CHECK_LAUNCH("kv8_attn");
   if (a.nshare == 1) return 0;

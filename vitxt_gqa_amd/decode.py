@@ -64,9 +64,9 @@ def _head_rows(t, name):
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_plan(B, N, H, G, max_len):
+def _attn_plan(B, N, H, G, max_len, dtype):
     """(shares of the token axis, bytes of workspace) of an attention over about ``max_len`` tokens."""
-    splits = X.lib().t2s_kv8_attn_splits(B, N, H, G, max_len)
+    splits = X.lib().t2s_kv8_attn_splits(B, N, H, G, max_len, dtype)
     return splits, X.lib().t2s_kv8_attn_workspace_bytes(B, N, H, G, splits)
 
 
@@ -191,8 +191,8 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
     [B, N] (all, without it; below 0 counts as 0, above T as T).  Returns (out [B, N, HQ, 64] in q's type, lse [B, N, HQ] float32: the natural
     log-sum-exp of the scaled scores).  A row that sees no token at all: out 0, lse -inf.
 
-    Codes enter the matrix pipe as exact bf16; a query in float32 as the three bf16 terms that make it up; probabilities as two terms (bfloat16
-    results: 16 bits, below the rounding of the result) or three (float32).  All sums, maxima and scales are float32; the result is rounded once."""
+    Codes enter the matrix pipe exactly; a query in float32 as the three bf16 terms that make it up; probabilities in 11 bits for a bfloat16
+    result (which is rounded to 8), as three bf16 terms for a float32 one.  All sums, maxima and scales are float32; the result is rounded once."""
     H = cache.heads
     if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[2] < 1 or q.shape[2] % H:
         _need(False, "attend: q [%d, N, a multiple of %d, 64], got %s", cache.batch, H, tuple(q.shape))
@@ -221,7 +221,7 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
     lse = torch.empty((B, N, HQ), dtype=torch.float32, device=q.device)
     if N == 0:
         return out, lse
-    splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len)
+    splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len, _DTYPES[q.dtype][0])
     ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
     X.check(_launch(cache._index, X.lib().t2s_kv8_attn, q.data_ptr(), sq[0], sq[1], sq[2], *cache._ptrs, tk, tv, st[0], st[1], st[2], st[3], tl, tls[0], tls[1], T,
                     out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, _DTYPES[q.dtype][0], cache._fmt), "t2s_kv8_attn")

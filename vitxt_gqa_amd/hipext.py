@@ -67,7 +67,7 @@ _SIGS = {
     "t2s_gemm_wgrad": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int64, c_int64, c_int, c_int, c_void_p]),
     "t2s_kv8_append": (c_int, [c_void_p] + [c_int64] * 3 + [c_void_p] + [c_int64] * 3 + [c_void_p, c_int64] + [c_void_p] * 7 + [c_int] * 7 + [c_void_p]),
     "t2s_kv8_dequantize": (c_int, [c_void_p] * 7 + [c_int] * 5 + [c_void_p]),
-    "t2s_kv8_attn_splits": (c_int, [c_int] * 5),
+    "t2s_kv8_attn_splits": (c_int, [c_int] * 6),
     "t2s_kv8_attn_workspace_bytes": (c_int64, [c_int] * 5),
     "t2s_kv8_attn": (c_int, [c_void_p] + [c_int64] * 3 + [c_void_p] * 7 + [c_int64] * 4 + [c_void_p, c_int64, c_int64, c_int] + [c_void_p] * 3 + [c_int64]
                      + [c_int] * 6 + [c_float, c_int, c_int, c_void_p]),
