@@ -18,6 +18,7 @@ import threading
 
 import torch
 
+from . import decode
 from . import gemm as own
 from . import ops
 
@@ -825,5 +826,64 @@ def encoder_decode_rows(x_dec, caches, keys, layers, dtype, row0):
         w = _layer_weights(lp, dtype)
         qkv[:, row0:row0 + D] = _mm_bias(xl, w[0], w[1]).view(B, D, 3 * HID)
         att = ops.attn_fwd_rows(qkv[:, row0:row0 + D, :HID], qkv, keys)
+        x2, xl = _layer_tail(att.view(B * D, HID), x2, w, dtype)
+    return x2.view(B, D, HID)
+
+
+# ---- the same with the prefix in 8 bits and one row per beam (T2S.set_decoding; operators: decode.py).  A step computes only its newest row:
+# a decoder row sees the prefix and the decoder rows up to itself (t2s.py:574-618), so the rows of earlier steps, whose K / V a beam keeps
+# in its tail, never change.
+@torch.no_grad()
+def encoder_prefill_kv8(x, keys, layers, dtype, fmt):
+    """Inference pass over the prefix rows alone.  x fp32 [B, L1, 768], ``keys`` its key list (no decoder rows).  Returns (out fp32 [B, L1, 768],
+    caches = per layer a decode.KVCache8 of the listed rows' K / V)."""
+    B, L, _ = x.shape
+    x2 = x.contiguous().view(B * L, HID)
+    xl = x2.to(dtype)
+    caches = []
+    for lp in layers:
+        w = _layer_weights(lp, dtype)
+        qkv = _mm_bias(xl, w[0], w[1]).view(B, L, 3 * HID)
+        att, _ = ops.attn_fwd(qkv, keys)
+        kv = qkv.view(B, L, 3, ops.HEADS, ops.HEAD_DIM)
+        cache = decode.KVCache8(B, ops.HEADS, keys.cap_hint, fmt, device=x.device)
+        caches.append(cache.append(kv[:, :, 1], kv[:, :, 2], counts=keys.cnt, rows=keys.idx))
+        x2, xl = _layer_tail(att.view(B * L, HID), x2, w, dtype)
+    return x2.view(B, L, HID), caches
+
+
+def kv8_tail(n_layers, B, N, steps, dtype, device):
+    """The decoded tokens' K | V of every layer and beam: [layers, B, N, steps, 2, 12, 64]."""
+    return torch.empty(n_layers, B, N, steps, 2, ops.HEADS, ops.HEAD_DIM, dtype=dtype, device=device)
+
+
+@torch.no_grad()
+def encoder_step_kv8(x, caches, tail, layers, dtype, t):
+    """Decoder row ``t`` of every beam: x fp32 [B, N, 768] (its layer-0 input) -> fp32 [B, N, 768].  Its K / V are put into ``tail``
+    (kv8_tail) at step t."""
+    B, N, _ = x.shape
+    x2 = x.contiguous().view(B * N, HID)
+    xl = x2.to(dtype)
+    for lp, cache, tl in zip(layers, caches, tail.unbind(0)):
+        w = _layer_weights(lp, dtype)
+        qkv = _mm_bias(xl, w[0], w[1]).view(B, N, 3, ops.HEADS, ops.HEAD_DIM)
+        tl[:, :, t] = qkv[:, :, 1:]
+        att, _ = decode.attend(qkv[:, :, 0], cache, tl[:, :, :, 0], tl[:, :, :, 1], t + 1)
+        x2, xl = _layer_tail(att.view(B * N, HID), x2, w, dtype)
+    return x2.view(B, N, HID)
+
+
+@torch.no_grad()
+def encoder_rows_kv8(x, caches, layers, dtype):
+    """All D decoder rows of one sequence at once: x fp32 [B, D, 768] -> fp32 [B, D, 768]; row i sees the prefix and rows 0 .. i."""
+    B, D, _ = x.shape
+    seen = torch.arange(1, D + 1, dtype=torch.int32, device=x.device).expand(B, D)
+    x2 = x.contiguous().view(B * D, HID)
+    xl = x2.to(dtype)
+    for lp, cache in zip(layers, caches):
+        w = _layer_weights(lp, dtype)
+        qkv = _mm_bias(xl, w[0], w[1]).view(B, D, 3, ops.HEADS, ops.HEAD_DIM)
+        shared = qkv.unsqueeze(1).expand(-1, D, -1, -1, -1, -1)             # every row reads the one tail
+        att, _ = decode.attend(qkv[:, :, 0], cache, shared[:, :, :, 1], shared[:, :, :, 2], seen)
         x2, xl = _layer_tail(att.view(B * D, HID), x2, w, dtype)
     return x2.view(B, D, HID)

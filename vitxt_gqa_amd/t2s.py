@@ -22,6 +22,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .gemm_tuning import enable_tuned_gemms
+from . import decode
 from . import functional as FN
 from . import ops
 from .base_model import BaseModel
@@ -267,13 +268,30 @@ class PrevPredEmbeddings(nn.Module):
         self.ocr_layer_norm = nn.LayerNorm(HID, eps=LN_EPS)
         self.emb_layer_norm = nn.LayerNorm(HID, eps=LN_EPS)
 
+    def step(self, ans_emb, ocr_emb, inds, t):
+        """The layer-0 input of decoding step ``t`` for each of N beams: inds [B, N] -> fp32 [B, N, 768] (forward's row t, no dropout)."""
+        is_ocr, raw = self._rows(ans_emb, ocr_emb, inds, 0)
+        emb = self.position_embeddings.weight[t] + self.token_type_embeddings(is_ocr.long())
+        return raw + FN.layer_norm(emb, self.emb_layer_norm.weight, self.emb_layer_norm.bias)
+
     def forward(self, ans_emb, ocr_emb, prev_inds, dtype, emb_dropout=0.0, draws=None, ocr_row0=0):
         """``draws`` = n: a list of n results that share the gathered rows and differ in the dropout draw of the position /
         type embedding only - the three MMT passes of a train step call this with the same inputs (t2s.py:293-313), and each
         separate call costs a [B, N, 768] zero fill + scatter + accumulation in the backward of its OCR-row gather."""
+        D = prev_inds.shape[1]
+        is_ocr, raw = self._rows(ans_emb, ocr_emb, prev_inds, ocr_row0)
+        emb = self.position_embeddings.weight[:D].unsqueeze(0) + self.token_type_embeddings(is_ocr.long())
+        emb = FN.layer_norm(emb, self.emb_layer_norm.weight, self.emb_layer_norm.bias)
+        if draws is not None:
+            return [raw + (F.dropout(emb, emb_dropout, True) if emb_dropout > 0 else emb) for _ in range(draws)]
+        if emb_dropout > 0:
+            emb = F.dropout(emb, emb_dropout, True)         # emb_dropout, t2s.py:720
+        return raw + emb
+
+    def _rows(self, ans_emb, ocr_emb, prev_inds, ocr_row0):
+        """(is_ocr [B, D], normalised rows fp32 [B, D, 768]) of the words and OCR slots ``prev_inds`` names."""
         # LayerNorm is row-wise, so LN(table)[gather] == LN(table[gather]): only the 12 gathered rows per
         # sample are normalised instead of the whole [V, 768] table + [B, N, 768] OCR tensor (t2s.py:702-709).
-        B, D = prev_inds.shape
         V = ans_emb.size(0)
         is_ocr = prev_inds.ge(V)
         ans_rows = ans_emb[prev_inds.clamp(max=V - 1)]                                            # [B, D, 768] fp32
@@ -284,14 +302,7 @@ class PrevPredEmbeddings(nn.Module):
         ocr_rows = torch.gather(ocr_emb, 1, ocr_idx.unsqueeze(-1).expand(-1, -1, HID))
         ans_n = FN.layer_norm(ans_rows, self.ans_layer_norm.weight, self.ans_layer_norm.bias)
         ocr_n = FN.layer_norm(ocr_rows, self.ocr_layer_norm.weight, self.ocr_layer_norm.bias)
-        raw = torch.where(is_ocr.unsqueeze(-1), ocr_n, ans_n)
-        emb = self.position_embeddings.weight[:D].unsqueeze(0) + self.token_type_embeddings(is_ocr.long())
-        emb = FN.layer_norm(emb, self.emb_layer_norm.weight, self.emb_layer_norm.bias)
-        if draws is not None:
-            return [raw + (F.dropout(emb, emb_dropout, True) if emb_dropout > 0 else emb) for _ in range(draws)]
-        if emb_dropout > 0:
-            emb = F.dropout(emb, emb_dropout, True)         # emb_dropout, t2s.py:720
-        return raw + emb
+        return is_ocr, torch.where(is_ocr.unsqueeze(-1), ocr_n, ans_n)
 
 
 class MMT(nn.Module):
@@ -442,6 +453,7 @@ class T2S(BaseModel):
         num_choices -= c.classifier.ocr_max_num
         self.classifier = _Classifier(HID, num_choices)
         self.answer_processor = registry.get(self._datasets[0] + "_answer_processor")
+        self.decode_beams, self.decode_cache = 1, None        # eval: see set_decoding
         self.decode_with_prefix_cache = True      # eval: reuse the step-invariant prefix K/V (False = reference's loop)
         # diagnostics for the parity tests: _last_fwd also keeps the pre-QTV encodings (txt_emb0 / obj_in0 / ocr_in0), and per MMT
         # pass the decoder-step embeddings and the encoder outputs ({ref,pos,neg}_dec_emb / _mmt_dec / _mmt_ocr)
@@ -495,6 +507,21 @@ class T2S(BaseModel):
         self.compute_dtype = dtype
         return self
 
+    def set_decoding(self, beams=1, cache=None):
+        """How eval decodes.  ``beams`` = 1, ``cache`` = None: the reference's greedy loop (t2s.py:315-354) with the prefix's K / V in the operand type.
+        ``cache`` = "int8" or "e4m3": the prefix in 8 bits (decode.KVCache8: half the memory and traffic of bf16), one new row per step.
+        ``beams`` > 1: beam search over the summed log-softmax of ``pos_scores`` (8-bit cache; "int8" unless said otherwise), a beam ending at
+        the answer processor's ``EOS_IDX`` if it has one; the output dict then also holds ``beam_tokens`` [B, beams, D] and ``beam_scores``
+        [B, beams], best first, and the three passes' scores are those along the best beam."""
+        if not 1 <= int(beams) <= 16:
+            raise ValueError("set_decoding: 1 to 16 beams, got %s" % (beams,))           # (the pointer kernel takes 16 rows a sample)
+        if cache is None and beams > 1:
+            cache = "int8"
+        if cache is not None and cache not in decode.FORMATS:
+            raise ValueError("set_decoding: unknown cache format %r (int8 or e4m3)" % (cache,))
+        self.decode_beams, self.decode_cache = int(beams), cache
+        return self
+
     # -- forward (t2s.py:153-354) ------------------------------------------------------------------
     def forward(self, sample_list):
         dt = self.compute_dtype
@@ -511,7 +538,8 @@ class T2S(BaseModel):
             self.Grounding_Module(sample_list, fwd)
             self._forward_mmt_and_output(sample_list, fwd, dt)
         self._last_fwd = fwd
-        return {"ref_scores": fwd["ref_scores"], "pos_scores": fwd["pos_scores"], "neg_scores": fwd["neg_scores"],
+        beams = {k: fwd[k] for k in ("beam_tokens", "beam_scores") if k in fwd}
+        return {**beams, "ref_scores": fwd["ref_scores"], "pos_scores": fwd["pos_scores"], "neg_scores": fwd["neg_scores"],
                 "ground_box": fwd["ground_bbox"], "ground_frame": fwd["ground_frame"],
                 "frame_topk": fwd["frame_topk"], "ocr_topk": fwd["ocr_topk"]}
 
@@ -590,6 +618,8 @@ class T2S(BaseModel):
         if self.training:
             fwd["prev_inds"] = s.train_prev_inds.clone()
             self._three_pass(fwd, fwd["prev_inds"], dt)
+        elif self.decode_cache is not None:
+            self._beam_decode(s, fwd, dt)
         elif not self.decode_with_prefix_cache:
             # the reference's loop verbatim (t2s.py:315-354): every step recomputes all three full MMT passes
             D = s.train_prev_inds.size(1)
@@ -644,6 +674,57 @@ class T2S(BaseModel):
             prev[:, 1:] = fwd["pos_scores"].argmax(dim=-1)[:, :-1]
         fwd["prev_inds"] = prev
         fwd["dec_emb_last"] = dec                                  # decoder-step embeddings of the last step (same for the 3 passes)
+
+    @torch.no_grad()
+    def _beam_decode(self, s, fwd, dt):
+        """Beam search over the "pos" pass, whose scores drive the reference's loop (t2s.py:315-354), on an 8-bit cache of its prefix: a step computes
+        the newest row of every beam, picks the best continuations of all beams and moves the beams' states to where they come from.  The
+        three passes' scores are then computed along the best beam, all decoder rows at once.  One beam: the greedy loop."""
+        g = self.Grounding_Module
+        txt, obj, ocr = fwd["txt_emb"], fwd["obj_mmt_in"], fwd["ocr_mmt_in"]
+        B, T, Fn, L1 = txt.size(0), txt.size(1), obj.size(1), txt.size(1) + obj.size(1) + ocr.size(1)
+        D, K, dev = s.train_prev_inds.size(1), self.decode_beams, txt.device
+        layers, pn, cls = self.mmt.encoder.layer, self.ocr_ptr_net, self.classifier.module
+        prefix = torch.cat([txt, obj, ocr], dim=1)
+        passes = {"ref": (fwd["obj_mask"], fwd["ocr_mask"], None),
+                  "pos": (fwd["pos_obj_mask"], fwd["pos_ocr_mask"], T + g.frame_topk + g.ocr_topk * g.frame_num),
+                  "neg": (fwd["neg_obj_mask"], fwd["neg_ocr_mask"], T + g.frame_topk + g.ocr_topk * g.frame_topk)}
+
+        def prefill(name):
+            om, cm, bound = passes[name]
+            keys = ops.compact_keys(torch.cat([fwd["txt_mask"] > 0, om > 0, cm > 0], dim=1), cap_hint=bound)
+            out, caches = FN.encoder_prefill_kv8(prefix, keys, layers, dt, self.decode_cache)
+            return caches, F.linear(out[:, T + Fn:L1].to(dt), pn.key.weight.to(dt), pn.key.bias.to(dt)).contiguous(), cm.float()
+
+        def scores(rows, k_ptr, cm):
+            return FN.ptr_logits(F.linear(rows, cls.weight, cls.bias), F.linear(rows, pn.query.weight, pn.query.bias), k_ptr, cm)
+
+        caches, k_ptr, cm = prefill("pos")
+        tail = FN.kv8_tail(len(layers), B, K, D, dt, dev)
+        eos = getattr(self.answer_processor, "EOS_IDX", None)
+        tokens = torch.full((B, K, D), 0, dtype=torch.int64, device=dev)
+        total = torch.full((B, K), -math.inf, device=dev)
+        total[:, 0] = 0.0                                          # every beam starts from the one that holds nothing yet
+        ended = None if eos is None else torch.zeros(B, K, dtype=torch.bool, device=dev)
+        last = torch.full((B, K), self.answer_processor.BOS_IDX, dtype=torch.int64, device=dev)
+        for t in range(D):
+            rows = FN.encoder_step_kv8(self.mmt.prev_pred_embeddings.step(cls.weight, ocr, last, t), caches, tail, layers, dt, t)
+            total, parents, last = decode.beam_select(scores(rows, k_ptr, cm), total, K, ended, eos or 0)
+            decode.beam_reorder(tokens, parents, used=t)
+            tokens[:, :, t] = last
+            if t + 1 < D:
+                decode.beam_reorder(tail, parents, batch_dim=1, used=t + 1)
+            if ended is not None:
+                ended = ended.gather(1, parents) | (last == eos)
+        prev = torch.cat([torch.full((B, 1), self.answer_processor.BOS_IDX, dtype=torch.int64, device=dev), tokens[:, 0, :-1]], dim=1)
+        dec = self.mmt.prev_pred_embeddings(cls.weight, ocr, prev, dt)
+        if self.keep_intermediates:
+            fwd["pos_caches"], fwd["pos_k_ptr"] = caches, k_ptr
+        for name in ("pos", "ref", "neg"):
+            if name != "pos":
+                caches, k_ptr, cm = prefill(name)
+            fwd[name + "_scores"] = scores(FN.encoder_rows_kv8(dec, caches, layers, dt), k_ptr, cm)
+        fwd["prev_inds"], fwd["beam_tokens"], fwd["beam_scores"] = prev, tokens, total
 
     # -- optimizer hook (t2s.py:356-376) -------------------------------------------------------------
     def get_optimizer_parameters(self, config):
