@@ -110,27 +110,85 @@ __device__ __forceinline__ f16x8 decode8_f16(uint32_t lo, uint32_t hi) {
 // word position of token group tg (tokens 4 tg .. 4 tg + 3) inside a value row: p / 4 of the order above
 __device__ __forceinline__ int v_word(int tg) { return (tg & 3) * 4 + (tg >> 2); }
 
+// lane exchanges without LDS: the pairs (x[l], x[l ^ 16]) and (x[l], x[l ^ 32]) in some order
+__device__ __forceinline__ void swap16(float x, float& a, float& b) {
+  const auto p = __builtin_amdgcn_permlane16_swap(as_u(x), as_u(x), false, false);
+  a = as_f(p[0]);
+  b = as_f(p[1]);
+}
+__device__ __forceinline__ void swap32(float x, float& a, float& b) {
+  const auto p = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
+  a = as_f(p[0]);
+  b = as_f(p[1]);
+}
+// maximum / sum over the four 16-lane groups that hold one query's keys
+__device__ __forceinline__ float across_max(float x) {
+  float a, b;
+  swap16(x, a, b);
+  swap32(fmaxf(a, b), a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float across_sum(float x) {
+  float a, b;
+  swap16(x, a, b);
+  swap32(a + b, a, b);
+  return a + b;
+}
+// value of lane l ^ 1 / l ^ 2 (quad permutes), l + 4 / l + 8 in a ring of 16 (row rotations)
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return as_f((uint32_t)__builtin_amdgcn_mov_dpp((int)as_u(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
+// maximum of an unsigned number over the wave
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  float a, b;
+  x = max(x, as_u(dpp<DPP_XOR1>(as_f(x))));
+  x = max(x, as_u(dpp<DPP_XOR2>(as_f(x))));
+  x = max(x, as_u(dpp<DPP_ROR4>(as_f(x))));
+  x = max(x, as_u(dpp<DPP_ROR8>(as_f(x))));
+  swap16(as_f(x), a, b);
+  swap32(as_f(max(as_u(a), as_u(b))), a, b);
+  return max(as_u(a), as_u(b));
+}
+// maximum / sum over the wave's sixteen quads, each of which holds one value four times
+__device__ __forceinline__ float quads_max(float x) {
+  x = fmaxf(x, dpp<DPP_ROR4>(x));
+  x = fmaxf(x, dpp<DPP_ROR8>(x));
+  return across_max(x);
+}
+__device__ __forceinline__ float quads_sum(float x) {
+  x += dpp<DPP_ROR4>(x);
+  x += dpp<DPP_ROR8>(x);
+  return across_sum(x);
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------------
-// append.  One workgroup = one (sequence, head, K or V) walking the blocks that the new tokens touch; a thread owns 4 tokens x 4 dims
-// of a block, so both storage orders are 32-bit words of it, and the words go out through a 4 KB LDS image as one contiguous block.
+// append.  One workgroup = one (sequence, head) walking the blocks that the new tokens touch; a thread owns 4 tokens x 4 dims of a block, of
+// keys and of values, so both storage orders are 32-bit words of it, and the words go out through LDS images as contiguous blocks.  HBM
+// bound: the rows of the next block are on their way (their numbers, where a list names them, one block further) while a block is encoded.
 struct AppendArgs {
   const void* x[2];                                // K, V
   int64_t x_bs[2], x_ts[2], x_hs[2];
   const int32_t *rows, *counts;
   int64_t rows_bs;
-  uint8_t *k8, *v8;
-  float *ks, *vs;
+  uint8_t* codes[2];
+  float* scales[2];
   int32_t *lens, *ticket;
   int B, H, T, L, nblk;
 };
 
 template <typename TX, int FMT>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
-  __shared__ __attribute__((aligned(16))) uint32_t img[KV_BYTES / 4];
-  __shared__ uint32_t red[4];
+  typedef TX Raw __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(16))) uint32_t img[2][KV_BYTES / 4];
+  __shared__ uint32_t red[2][4];
   const int tid = threadIdx.x, tg = tid >> 4, dg = tid & 15;
-  const int which = blockIdx.y & 1, h = blockIdx.y >> 1, b = blockIdx.z;
+  const int h = blockIdx.y, b = blockIdx.z;
   const int len = a.lens[b];
+  // A workgroup draws a ticket of its sequence once all of its waves have read the length (behind its first barrier: the ticket is on its way
+  // while the block is encoded); the one with the last ticket advances the length at its end.
+  int ticket = 0;
   const int cap = a.nblk * KV_BLOCK;
   int n = a.counts ? a.counts[b] : a.T;
   n = n < 0 ? 0 : (n > a.T ? a.T : n);
@@ -138,88 +196,119 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
   const int room = poisoned ? 0 : cap - len;
   const bool over = n > room;
   if (over) n = room;
+  int begin = 0;
+  bool idle = true;
   if (!poisoned && n > 0) {
-    const TX* x = (const TX*)a.x[which] + (int64_t)b * a.x_bs[which] + (int64_t)h * a.x_hs[which] + dg * 4;
-    const int64_t x_ts = a.x_ts[which];
+    const TX* x[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) x[w] = (const TX*)a.x[w] + (int64_t)b * a.x_bs[w] + (int64_t)h * a.x_hs[w] + dg * 4;
+    const int32_t* rows = a.rows ? a.rows + (int64_t)b * a.rows_bs : nullptr;
     const int64_t base = ((int64_t)b * a.H + h) * a.nblk;
-    uint8_t* codes = which ? a.v8 : a.k8;
-    float* scales = which ? a.vs : a.ks;
-    const int first = len / KV_BLOCK, last = (len + n - 1) / KV_BLOCK;
-    for (int blk = first + blockIdx.x; blk <= last; blk += gridDim.x) {
-      uint8_t* dst = codes + (base + blk) * KV_BYTES;
-      const bool joins = blk == first && len % KV_BLOCK != 0;          // the block holds tokens already
-      const float s_old = joins ? scales[base + blk] : 0.f;
-      float val[4][4];                                                  // [token][dim]
-      uint32_t mx = 0;
+    const int first = len / KV_BLOCK, last = (len + n - 1) / KV_BLOCK, stride = gridDim.x;
+    // row numbers of this thread's four tokens of a block: -1 where there is no new token, L where the list names a row that is not there
+    auto numbers = [&](int blk, int (&r)[4]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int j = blk * KV_BLOCK + tg * 4 + i - len;               // number of the new token
-        f32x4 f = {0.f, 0.f, 0.f, 0.f};
+        const int j = blk * KV_BLOCK + tg * 4 + i - len;
+        r[i] = -1;
         if (j >= 0 && j < n) {
-          int64_t row = a.rows ? a.rows[(int64_t)b * a.rows_bs + j] : j;
-          if (row >= 0 && row < a.L) f = Vec4<TX>::load(x + row * x_ts);
-          else f[0] = as_f(0x7fc00000u);                                // a row that is not there: the block turns NaN
-        }
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          val[i][d] = f[d];
-          mx = max(mx, as_u(f[d]) & 0x7fffffffu);
+          r[i] = rows ? rows[j] : j;
+          if (r[i] < 0 || r[i] > a.L) r[i] = a.L;
         }
       }
+    };
+    auto fetch = [&](const int (&r)[4], Raw (&d)[2][4]) {
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o, 64));
-      if ((tid & 63) == 0) red[tid >> 6] = mx;
-      if (joins) {                                                      // what the block holds, read before anyone writes (barrier below)
-        const uint32_t* src = (const uint32_t*)dst;
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float old[4];
-          if (which == 0) {
-            decode4<FMT>(src[(tg * 4 + i) * 16 + dg], old);             // token tg * 4 + i, four dims
-            if (blk * KV_BLOCK + tg * 4 + i < len)
+          d[w][i] = Raw{(TX)0.f, (TX)0.f, (TX)0.f, (TX)0.f};
+          if (r[i] >= 0 && r[i] < a.L) d[w][i] = *(const Raw*)(x[w] + r[i] * a.x_ts[w]);
+          else if (r[i] >= a.L) d[w][i][0] = (TX)as_f(0x7fc00000u);    // a row that is not there: the block turns NaN
+        }
+    };
+    int r_next[4];
+    Raw d_next[2][4];
+    begin = first + blockIdx.x;
+    idle = begin > last;
+    int blk = begin;
+    if (blk <= last) {
+      numbers(blk, r_next);
+      fetch(r_next, d_next);
+      if (blk + stride <= last) numbers(blk + stride, r_next);
+    }
+    for (; blk <= last; blk += stride) {
+      const bool joins = blk == first && len % KV_BLOCK != 0;          // the block holds tokens already
+      float val[2][4][4];                                               // [K, V][token][dim]
 #pragma unroll
-              for (int d = 0; d < 4; ++d) val[i][d] = old[d] * s_old;
-          } else {
-            decode4<FMT>(src[(dg * 4 + i) * 16 + v_word(tg)], old);     // dim dg * 4 + i, four tokens
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-              if (blk * KV_BLOCK + tg * 4 + t < len) val[t][i] = old[t] * s_old;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) val[w][i][d] = (float)d_next[w][i][d];
+      if (blk + stride <= last) {
+        fetch(r_next, d_next);
+        if (blk + 2 * stride <= last) numbers(blk + 2 * stride, r_next);
+      }
+      float s_old[2] = {0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        uint32_t mx = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) mx = max(mx, as_u(val[w][i][d]) & 0x7fffffffu);
+        mx = wave_max(mx);
+        if ((tid & 63) == 0) red[w][tid >> 6] = mx;
+        if (joins) {                                                    // what the block holds, read before anyone writes (barrier below)
+          const uint32_t* src = (const uint32_t*)(a.codes[w] + (base + blk) * KV_BYTES);
+          s_old[w] = a.scales[w][base + blk];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float old[4];
+            if (w == 0) {
+              decode4<FMT>(src[(tg * 4 + i) * 16 + dg], old);           // token tg * 4 + i, four dims
+              if (blk * KV_BLOCK + tg * 4 + i < len)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) val[w][i][d] = old[d] * s_old[w];
+            } else {
+              decode4<FMT>(src[(dg * 4 + i) * 16 + v_word(tg)], old);   // dim dg * 4 + i, four tokens
+#pragma unroll
+              for (int t = 0; t < 4; ++t)
+                if (blk * KV_BLOCK + tg * 4 + t < len) val[w][t][i] = old[t] * s_old[w];
+            }
           }
         }
       }
       __syncthreads();
-      mx = max(max(red[0], red[1]), max(red[2], red[3]));
-      float s = scale_of<FMT>(mx);
-      if (joins && !(s >= s_old)) s = s != s ? s : s_old;               // the larger of the two; a NaN on either side stays
-      const float r = s == s ? 1.0f / s : 0.f;
-      if (s != s)
+      if (tid == 0 && blk == begin) ticket = atomicAdd(a.ticket + b, 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t mx = max(max(red[w][0], red[w][1]), max(red[w][2], red[w][3]));
+        float s = scale_of<FMT>(mx);
+        if (joins && !(s >= s_old[w])) s = s != s ? s : s_old[w];       // the larger of the two; a NaN on either side stays
+        const float r = s == s ? 1.0f / s : 0.f;
 #pragma unroll
-          for (int d = 0; d < 4; ++d) val[i][d] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (which == 0) {
-          img[(tg * 4 + i) * 16 + dg] = encode4<FMT>(val[i], r);
-        } else {
-          const float col[4] = {val[0][i], val[1][i], val[2][i], val[3][i]};
-          img[(dg * 4 + i) * 16 + v_word(tg)] = encode4<FMT>(col, r);
+        for (int i = 0; i < 4; ++i) {
+          const float col[4] = {val[w][0][i], val[w][1][i], val[w][2][i], val[w][3][i]};
+          const uint32_t code = s == s ? encode4<FMT>(w == 0 ? val[w][i] : col, r) : 0u;
+          img[w][w == 0 ? (tg * 4 + i) * 16 + dg : (dg * 4 + i) * 16 + v_word(tg)] = code;
         }
+        if (tid == 0) a.scales[w][base + blk] = s;
       }
       __syncthreads();
-      ((uint4*)dst)[tid] = ((const uint4*)img)[tid];
-      if (tid == 0) scales[base + blk] = s;
-      // (the next round's barrier after `red` keeps its image writes behind this round's reads)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) ((uint4*)(a.codes[w] + (base + blk) * KV_BYTES))[tid] = ((const uint4*)img[w])[tid];
+      // (the next round's barrier behind `red` keeps its image writes behind this round's reads)
     }
   }
-  // the sequence's last workgroup advances its length: every other one has read it before it drew its ticket
-  __syncthreads();
-  if (tid == 0) {
-    const int total = (int)(gridDim.x * gridDim.y);
-    if (atomicAdd(a.ticket + b, 1) == total - 1) {
-      a.ticket[b] = 0;
-      a.lens[b] = poisoned || over ? -1 : len + n;
-    }
+  if (idle) {
+    __syncthreads();
+    if (tid == 0) ticket = atomicAdd(a.ticket + b, 1);
+  }
+  if (tid == 0 && ticket == (int)(gridDim.x * gridDim.y) - 1) {
+    a.ticket[b] = 0;
+    a.lens[b] = poisoned || over ? -1 : len + n;
   }
 }
 
@@ -296,48 +385,6 @@ __device__ __forceinline__ void split_bf16(float x, bf16_t (&o)[TERMS]) {
     o[i] = (bf16_t)x;
     x -= (float)o[i];
   }
-}
-
-// lane exchanges without LDS: the pairs (x[l], x[l ^ 16]) and (x[l], x[l ^ 32]) in some order
-__device__ __forceinline__ void swap16(float x, float& a, float& b) {
-  const auto p = __builtin_amdgcn_permlane16_swap(as_u(x), as_u(x), false, false);
-  a = as_f(p[0]);
-  b = as_f(p[1]);
-}
-__device__ __forceinline__ void swap32(float x, float& a, float& b) {
-  const auto p = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
-  a = as_f(p[0]);
-  b = as_f(p[1]);
-}
-// maximum / sum over the four 16-lane groups that hold one query's keys
-__device__ __forceinline__ float across_max(float x) {
-  float a, b;
-  swap16(x, a, b);
-  swap32(fmaxf(a, b), a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float across_sum(float x) {
-  float a, b;
-  swap16(x, a, b);
-  swap32(a + b, a, b);
-  return a + b;
-}
-// value of lane l ^ 1 / l ^ 2 (quad permutes), l + 4 / l + 8 in a ring of 16 (row rotations)
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return as_f((uint32_t)__builtin_amdgcn_mov_dpp((int)as_u(x), CTRL, 0xf, 0xf, true));
-}
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
-// maximum / sum over the wave's sixteen quads, each of which holds one value four times
-__device__ __forceinline__ float quads_max(float x) {
-  x = fmaxf(x, dpp<DPP_ROR4>(x));
-  x = fmaxf(x, dpp<DPP_ROR8>(x));
-  return across_max(x);
-}
-__device__ __forceinline__ float quads_sum(float x) {
-  x += dpp<DPP_ROR4>(x);
-  x += dpp<DPP_ROR8>(x);
-  return across_sum(x);
 }
 
 // The second product of a block: V^T P^T, codes times probabilities, for the tokens of step s of a lane.  A bf16 result takes its
@@ -752,6 +799,10 @@ void launch_join(const AttnArgs& a, hipStream_t st) {
 // of 12, 16 sequences: 17.1 us in one launch, 14.3 with workgroups for the tails and a join; 5 rows: 12.9 and 14.1)
 constexpr int DIRECT_ROWS = 8;
 
+// Workgroups of an append (each draws a ticket of its sequence).  64 x 12 pairs of 7 000 tokens, us: 2 048 565, 6 144 490, 16 384 461 - 4.5 TB/s,
+// what a large copy reaches.
+constexpr int APPEND_WGS = 16384;
+
 bool kv8_bad_fmt(int fmt) { return fmt != FMT_INT8 && fmt != FMT_E4M3; }
 
 // Row groups of a (sequence, head), each of which reads its cache: as few as registers allow (64 rows; fp32, with three terms to everything,
@@ -778,14 +829,14 @@ extern "C" int t2s_kv8_append(const void* k, int64_t k_batch_stride, int64_t k_r
                     v_batch_stride % 4 == 0 && v_row_stride % 4 == 0 && v_head_stride % 4 == 0,
                 "kv8_append: rows must be aligned to 4 elements");
   T2S_CHECK_ARG((uintptr_t)k8 % 16 == 0 && (uintptr_t)v8 % 16 == 0, "kv8_append: the cache must be aligned to 16 bytes");
-  AppendArgs a{{k, v}, {k_batch_stride, v_batch_stride}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride}, rows, counts, rows_batch_stride, (uint8_t*)k8, (uint8_t*)v8,
-               k_scale, v_scale, lens, ticket, B, H, T, L, nblk};
+  AppendArgs a{{k, v}, {k_batch_stride, v_batch_stride}, {k_row_stride, v_row_stride}, {k_head_stride, v_head_stride}, rows, counts, rows_batch_stride, {(uint8_t*)k8, (uint8_t*)v8},
+               {k_scale, v_scale}, lens, ticket, B, H, T, L, nblk};
   const int touched = (int)((T + 62LL) / 64 + 1);
   // enough workgroups to fill the card (8 of them run on a CU), no more: each draws a ticket of its sequence when it ends
-  const int64_t pairs = (int64_t)B * H * 2;
-  int64_t gx = (8192 + pairs - 1) / pairs;
+  const int64_t pairs = (int64_t)B * H;
+  int64_t gx = (APPEND_WGS + pairs - 1) / pairs;
   if (gx > touched) gx = touched;
-  dim3 grid((unsigned)gx, (unsigned)(2 * H), (unsigned)B), block(256);
+  dim3 grid((unsigned)gx, (unsigned)H, (unsigned)B), block(256);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == T2S_BF16 && fmt == FMT_INT8) hipLaunchKernelGGL((kv8_append_kernel<bf16_t, FMT_INT8>), grid, block, 0, st, a);
   else if (dtype == T2S_BF16) hipLaunchKernelGGL((kv8_append_kernel<bf16_t, FMT_E4M3>), grid, block, 0, st, a);
