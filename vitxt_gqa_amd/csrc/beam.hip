@@ -12,14 +12,19 @@
 // holds a stretch of a row in registers, keeps its running maximum / sum of exponentials and its `select` best keys; a second kernel
 // joins the stretches of a sequence and orders the candidates of its N rows by their scores in 64 bits (rows differ by
 // cum - log-sum-exp, which 32 bits would merge into false ties).
+#include <algorithm>
+
 #include "common.h"
+#include "lanes.h"
 
 namespace {
 
 constexpr int BS_MAX = T2S_BEAM_MAX;               // beams, and candidates to select
 constexpr int BS_EPT = 16;                         // elements of a thread per stretch
 constexpr int BS_SUB = 256 * BS_EPT;
-constexpr int BS_CHUNKS = 32;                      // stretches of a row at most; longer ones walk several in turn
+constexpr int BS_CHUNKS = 32;                      // workgroups of a row at most
+constexpr int BS_WGS = 2048;
+constexpr int BS_LIST = 256;                       // logits of a wave that are ranked without more ado
 
 // order-preserving unsigned form of a float (-inf < ... < -0 = +0 < ... < max)
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -32,10 +37,10 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
 // NaN counts as a masked word, +inf as the largest number
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
 
-// VEC consecutive logits; past the row's end: -inf.  `whole`: rows that start at 16-byte boundaries.
+// VEC consecutive logits of a row from x[v] on, x + v at a 16-byte boundary; before the row's start and past its end: -inf
 template <typename TX, int VEC>
-__device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v, int V, bool whole, float* o) {
-  if (whole && v + VEC <= V) {
+__device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v, int V, float* o) {
+  if (v >= 0 && v + VEC <= V) {
 #pragma unroll
     for (int i = 0; i < VEC; i += 4) {
       const f32x4 f = Vec4<TX>::load(x + v + i);
@@ -44,20 +49,20 @@ __device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v,
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = v + i < V ? clean((float)x[v + i]) : -INFINITY;
+    for (int i = 0; i < VEC; ++i) o[i] = v + i >= 0 && v + i < V ? clean((float)x[v + i]) : -INFINITY;
   }
 }
 
-// a bound that the K largest of a wave's 64 keys reach and, where keys are unique, no others do; 1 where fewer than K are not zero.  Bit by
-// bit from the top, the lanes at or above a trial value counted by a ballot; done as soon as exactly K are left (some 20 steps on
-// random logits, 64 at most)
+// A bound that the K largest of a wave's 64 keys reach and, where keys are unique, no others do; 1 where fewer than K are not zero.  Two bits
+// at a time from the top, the lanes at or above the three trial values counted by ballots; done as soon as exactly K are left (some 10
+// steps on random logits, 32 at most)
 __device__ __forceinline__ uint64_t wave_kth(uint64_t key, int K) {
   uint64_t t = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t trial = t | 1ull << bit;
-    const int c = __popcll(__ballot(key >= trial));
-    if (c >= K) t = trial;
-    if (c == K) break;
+  for (int bit = 62; bit >= 0; bit -= 2) {
+    const uint64_t t1 = t | 1ull << bit, t2 = t | 2ull << bit, t3 = t | 3ull << bit;
+    const int c1 = __popcll(__ballot(key >= t1)), c2 = __popcll(__ballot(key >= t2)), c3 = __popcll(__ballot(key >= t3));
+    t = c3 >= K ? t3 : c2 >= K ? t2 : c1 >= K ? t1 : t;
+    if (c1 == K || c2 == K || c3 == K) break;
   }
   return t ? t : 1;
 }
@@ -66,52 +71,61 @@ template <typename TX>
 __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ logits, int64_t l_bs, int64_t l_ns, const float* __restrict__ cum,
                                                         const uint8_t* __restrict__ finished, uint64_t* __restrict__ keys, double* __restrict__ sums,
                                                         float* __restrict__ maxs, int N, int V, int K, int pad, int chunks, int subs) {
-  constexpr int VEC = 16 / sizeof(TX), SEG = BS_MAX * (BS_EPT + 1);
-  __shared__ uint64_t list_s[4][SEG];
-  __shared__ uint64_t top_s[BS_MAX], thr_s[4];
-  __shared__ int cnt_s[4];
+  constexpr int VEC = 16 / sizeof(TX);
+  __shared__ uint64_t list_s[4 * BS_MAX * (BS_EPT + 1)];
+  __shared__ uint64_t top_s[BS_MAX];
+  __shared__ uint32_t low_s[4];
+  __shared__ int cnt_s;
   __shared__ float m_s[4];
   __shared__ double s_s[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, chunk = blockIdx.x % chunks;
   const int64_t row = blockIdx.x / chunks;
   const int b = (int)(row / N), n = (int)(row % N);
   const TX* x = logits + (int64_t)b * l_bs + (int64_t)n * l_ns;
-  const bool whole = (uintptr_t)x % 16 == 0;
+  // stretches begin at 16-byte boundaries: `skew` elements before the row's first one
+  const int skew = (int)((uintptr_t)x % 16 / sizeof(TX));
+  // the first logits are on their way before it is known whether the row's are wanted at all
+  float val[BS_EPT];
+#pragma unroll
+  for (int i = 0; i < BS_EPT; i += VEC) load_logits<TX, VEC>(x, (int64_t)chunk * subs * BS_SUB - skew + i * 256 + tid * VEC, V, val + i);
   const float c = cum[row];
   const bool dead = !(c > -INFINITY);                                  // -inf or NaN: every candidate of the row is -inf
   const bool ended = finished && finished[row];
-  const bool virt = dead || ended;                                     // nothing of the row's logits is read
-  const int only = dead ? -1 : pad;                                    // an ended row offers `pad` at its own score
+  const int64_t out_at = row * chunks + chunk;
+  auto key_of = [](float x, int64_t v) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - (uint32_t)v); };
+  if (dead || ended) {
+    // nothing of the row's logits counts: an ended row offers `pad` at its own score; all else is at -inf, the lowest words first
+    if (tid < K) {
+      const int v = dead ? tid : tid - 1 + (tid - 1 >= pad ? 1 : 0);
+      keys[out_at * K + tid] = chunk != 0 ? 0 : ended && !dead && tid == 0 ? key_of(0.f, pad) : v < V ? key_of(-INFINITY, v) : 0;
+    }
+    if (tid == 0) {
+      maxs[out_at] = -INFINITY;
+      sums[out_at] = 0.0;
+    }
+    return;
+  }
   if (tid < BS_MAX) top_s[tid] = 0;
   float m = -INFINITY;
   double sum = 0.0;
   for (int sub = chunk * subs; sub < (chunk + 1) * subs; ++sub) {
-    const int64_t v0 = (int64_t)sub * BS_SUB;
+    const int64_t v0 = (int64_t)sub * BS_SUB - skew;
     if (v0 >= V) break;
-    // of a row without logits only its first words (all -inf, lowest index first) and `pad` can be selected
-    if (virt && sub != 0 && !(only >= v0 && only < v0 + BS_SUB)) continue;
-    float val[BS_EPT];
+    if (sub != chunk * subs)
 #pragma unroll
-    for (int i = 0; i < BS_EPT; i += VEC) {
-      const int64_t v = v0 + i * 256 + tid * VEC;
-      if (!virt) {
-        load_logits<TX, VEC>(x, v, V, whole, val + i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) val[i + j] = v + j == only ? 0.f : -INFINITY;
-      }
-    }
+      for (int i = 0; i < BS_EPT; i += VEC) load_logits<TX, VEC>(x, v0 + i * 256 + tid * VEC, V, val + i);
     auto index = [&](int i) { return v0 + (i / VEC) * VEC * 256 + tid * VEC + i % VEC; };       // rises with i
-    auto key_of = [&](float x, int64_t v) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - (uint32_t)v); };
-    float mx = val[0];
-    int at = 0;
+    float mx = -INFINITY;
+    int at = index(0) < 0 ? (int)-index(0) : 0;                          // (the first that is of the row)
 #pragma unroll
-    for (int i = 1; i < BS_EPT; ++i)
+    for (int i = 0; i < BS_EPT; ++i)
       if (val[i] > mx) {
         mx = val[i];
         at = i;
       }
-    uint64_t best = index(0) < V ? key_of(mx, index(at)) : 0;
+    // index(at) where `at` is a run-time value: the elements of a lane are VEC apart from the next ones of 256 lanes
+    const int64_t v_at = v0 + (at / VEC) * VEC * 256 + tid * VEC + at % VEC;
+    uint64_t best = v_at < V ? key_of(mx, v_at) : 0;
     if (mx > m) {
       sum *= (double)__expf(m - mx);
       m = mx;
@@ -122,70 +136,85 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
       for (int i = 0; i < BS_EPT; ++i) s += __expf(val[i] - m);
       sum += (double)s;
     }
-    // ---- the K best of (this stretch, what is kept of the former ones).  The K-th largest of a wave's best keys, one a lane, bounds the
-    // stretch's K-th largest key from below; so does the largest such bound of the four waves.  Of a wave's lanes at most K reach its own
-    // bound, so at most K (BS_EPT + 1) of its keys are listed - on random logits hardly more than K of all four.
+    // ---- the K best of (this stretch, what is kept of the former ones).  A number that K lanes' best logits reach bounds the K-th largest from
+    // below; the largest such number of the four waves, or the K-th of what is kept already, leaves little more than K logits to rank.
     __syncthreads();
     const uint64_t kept = tid < K ? top_s[tid] : 0;
-    best = kept > best ? kept : best;
-    const uint64_t own = wave_kth(best, K);
-    if (lane == 0) thr_s[wave] = own;
+    const uint32_t low = max(wave_kth_bound(ordered(mx), K), (uint32_t)(top_s[K - 1] >> 32));
+    if (lane == 0) low_s[wave] = low;
+    if (tid == 0) cnt_s = 0;
     __syncthreads();
-    uint64_t thr = thr_s[0];
+    // (below -inf's form there is no number: everything passes)
+    const uint32_t low4 = max(max(low_s[0], low_s[1]), max(low_s[2], low_s[3]));
+    const float tv = low4 > 0x7fffffu ? from_ordered(low4) : -INFINITY;
+    uint32_t mask = 0;                                                  // this lane's logits that reach it
+    int cnt = __popcll(__ballot(kept != 0));
 #pragma unroll
-    for (int w = 1; w < 4; ++w) thr = thr_s[w] > thr ? thr_s[w] : thr;
-    // (a bound found early is the upper bits of a key: below those of -inf it is no number, and everything passes)
-    const float tv = thr >> 32 > 0x7fffffu ? from_ordered((uint32_t)(thr >> 32)) : -INFINITY;
-    int cnt = 0;                                                        // of this wave
+    for (int i = 0; i < BS_EPT; ++i) {
+      const bool in = val[i] >= tv;
+      cnt += __popcll(__ballot(in));
+      mask |= in ? 1u << i : 0u;
+    }
+    // Many of them (logits in an order that defeats the bound, equal ones, lanes without any): only those that reach the wave's K-th best
+    // of one key a lane, at most K (BS_EPT + 1); those are unique.
+    uint64_t thr = 1;
+    if (cnt > BS_LIST) {
+      thr = wave_kth(kept > best ? kept : best, K);
+      cnt = __popcll(__ballot(kept >= thr));
+      mask = 0;
 #pragma unroll
-    for (int i = 0; i < BS_EPT; ++i)
-      if (__ballot(val[i] >= tv)) {
-        const uint64_t k = key_of(val[i], index(i));
-        const bool in = index(i) < V && k >= thr;
-        const uint64_t who = __ballot(in);
-        if (in) list_s[wave][cnt + __popcll(who & ((1ull << lane) - 1))] = k;
-        cnt += __popcll(who);
+      for (int i = 0; i < BS_EPT; ++i) {
+        const bool in = index(i) >= 0 && index(i) < V && key_of(val[i], index(i)) >= thr;
+        cnt += __popcll(__ballot(in));
+        mask |= in ? 1u << i : 0u;
       }
-    const uint64_t who = __ballot(kept >= thr);
-    if (kept >= thr) list_s[wave][cnt + __popcll(who & ((1ull << lane) - 1))] = kept;
-    cnt += __popcll(who);
-    if (lane == 0) cnt_s[wave] = cnt;
+    }
+    int to = 0;
+    if (lane == 0 && cnt) to = atomicAdd(&cnt_s, cnt);
+    to = __builtin_amdgcn_readfirstlane(to);
+    const int end = to + cnt;
+    {
+      const uint64_t who = __ballot(kept >= thr);
+      if (kept >= thr) list_s[to + __popcll(who & ((1ull << lane) - 1))] = kept;
+      to += __popcll(who);
+    }
+    for (uint64_t who = __ballot(mask != 0); who; who = __ballot(mask != 0)) {
+      const int i = __builtin_ctz(mask | 1u << BS_EPT);
+      float x = val[0];
+#pragma unroll
+      for (int j = 1; j < BS_EPT; ++j) x = i == j ? val[j] : x;
+      const int64_t v = v0 + (i / VEC) * VEC * 256 + tid * VEC + i % VEC;
+      if (mask) list_s[to + __popcll(who & ((1ull << lane) - 1))] = v >= 0 && v < V ? key_of(x, v) : 0;
+      mask &= mask - 1;
+      to += __popcll(who);
+    }
+    for (int i = to + lane; i < end; i += 64) list_s[i] = 0;
     __syncthreads();
-    const int c0 = cnt_s[0], c1 = c0 + cnt_s[1], c2 = c1 + cnt_s[2], c3 = c2 + cnt_s[3];
-    for (int i = tid; i < c3; i += 256) {
-      const int w = (i >= c0) + (i >= c1) + (i >= c2);
-      const uint64_t mine = list_s[w][i - (w == 0 ? 0 : w == 1 ? c0 : w == 2 ? c1 : c2)];
+    const int total = cnt_s;
+    for (int i = tid; i < total; i += 256) {
+      const uint64_t mine = list_s[i];
       int rank = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int n_u = u == 0 ? c0 : u == 1 ? c1 - c0 : u == 2 ? c2 - c1 : c3 - c2;
-#pragma unroll 4
-        for (int j = 0; j < n_u; ++j) rank += list_s[u][j] > mine;
-      }
-      if (rank < K) top_s[rank] = mine;
+#pragma unroll 8
+      for (int j = 0; j < total; ++j) rank += list_s[j] > mine;
+      if (rank < K) top_s[rank] = mine;                                  // (empty places rank behind all keys)
     }
   }
   // ---- the row's maximum and sum over this workgroup
-  float mw = m;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) mw = fmaxf(mw, __shfl_xor(mw, o, 64));
-  double sw = m > -INFINITY ? sum * (double)__expf(m - mw) : 0.0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sw += __shfl_xor(sw, o, 64);
-  if ((tid & 63) == 0) {
-    m_s[tid >> 6] = mw;
-    s_s[tid >> 6] = sw;
+  const float mw = wave_max(m);
+  const double sw = wave_sum64(m > -INFINITY ? sum * (double)__expf(m - mw) : 0.0);
+  if (lane == 0) {
+    m_s[wave] = mw;
+    s_s[wave] = sw;
   }
   __syncthreads();
-  const int64_t at = row * chunks + chunk;
-  if (tid < K) keys[at * K + tid] = top_s[tid];
+  if (tid < K) keys[out_at * K + tid] = top_s[tid];
   if (tid == 0) {
     const float m4 = fmaxf(fmaxf(m_s[0], m_s[1]), fmaxf(m_s[2], m_s[3]));
     double s4 = 0.0;
     for (int w = 0; w < 4; ++w)
       if (m_s[w] > -INFINITY) s4 += s_s[w] * (double)__expf(m_s[w] - m4);
-    maxs[at] = m4;
-    sums[at] = s4;
+    maxs[out_at] = m4;
+    sums[out_at] = s4;
   }
 }
 
@@ -207,8 +236,8 @@ __device__ __forceinline__ uint64_t ordered64(double x) {
 __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restrict__ keys, const double* __restrict__ sums, const float* __restrict__ maxs,
                                                         const float* __restrict__ cum, const uint8_t* __restrict__ finished, float* __restrict__ out_scores,
                                                         int64_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens, int N, int K, int chunks) {
-  __shared__ double off_s[BS_MAX];
-  __shared__ float top_m[BS_MAX];
+  __shared__ double off_s[BS_MAX], part_s[BS_MAX * BS_CHUNKS];
+  __shared__ float top_m[BS_MAX], part_m[BS_MAX * BS_CHUNKS];
   __shared__ Cand list_s[256 * BJ_PER + BS_MAX], top_s[BS_MAX];
   __shared__ uint64_t thr_s[4];
   __shared__ int cnt_s;
@@ -220,20 +249,23 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
   uint64_t raw[BJ_PER];                            // (in flight beside the rows' sums)
 #pragma unroll
   for (int j = 0; j < BJ_PER; ++j) raw[j] = tid + j * 256 < M ? kb[tid + j * 256] : 0;
+  for (int i = tid; i < N * chunks; i += 256) {
+    part_m[i] = maxs[(int64_t)b * N * chunks + i];
+    part_s[i] = sums[(int64_t)b * N * chunks + i];
+  }
+  const int64_t row = (int64_t)b * N + min(tid, N - 1);
+  const float c0 = cum[row];
+  const bool ended = finished && finished[row];
+  __syncthreads();
   if (tid < N) {
-    const int64_t row = (int64_t)b * N + tid;
-    const float c = cum[row];
-    const bool ended = finished && finished[row];
-    float m = -INFINITY;
+    float m = part_m[tid * chunks];
+    for (int i = 1; i < chunks; ++i) m = fmaxf(m, part_m[tid * chunks + i]);
     double s = 0.0;
-#pragma unroll 4
     for (int i = 0; i < chunks; ++i) {
-      const float mi = maxs[row * chunks + i], mn = fmaxf(m, mi);
-      const double si = sums[row * chunks + i];
-      if (mn > -INFINITY) s = s * (double)__expf(m - mn) + si * (double)__expf(mi - mn);
-      m = mn;
+      const float mi = part_m[tid * chunks + i];
+      if (mi > -INFINITY) s += part_s[tid * chunks + i] * (double)__expf(mi - m);
     }
-    const double cd = c > -INFINITY ? (double)fminf(c, 3.402823466e38f) : -INFINITY;
+    const double cd = c0 > -INFINITY ? (double)fminf(c0, 3.402823466e38f) : -INFINITY;
     top_m[tid] = ended ? 0.f : m;
     off_s[tid] = ended || !(s > 0.0) ? cd : cd - log(s);
   }
@@ -259,12 +291,12 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
     // a lower bound for the K-th best score, as in the rows' kernel; equal scores are all listed (the list holds everything there is)
     if (tid == 0) cnt_s = 0;
     uint64_t thr = 1;
-    if (M > 256) {
+    if (M > 64) {
       thr = wave_kth(best, K);
       if (lane == 0) thr_s[tid >> 6] = thr;
     }
     __syncthreads();
-    if (M > 256)
+    if (M > 64)
       for (int w = 0; w < 4; ++w) thr = max(thr, thr_s[w]);
     if (best >= thr) {
 #pragma unroll
@@ -333,10 +365,12 @@ int launch_reorder(void* state, const int64_t* parents, int outer, int B, int N,
   return 0;
 }
 
-// stretches of a row, and how many sub-stretches each walks
-void beam_chunks(int V, int* chunks, int* subs) {
-  const int n = (int)(((int64_t)V + BS_SUB - 1) / BS_SUB);
-  *subs = (n + BS_CHUNKS - 1) / BS_CHUNKS;
+// Workgroups of a row and the stretches each walks: one stretch each while that makes no more than BS_WGS workgroups (later stretches are
+// cheaper, they have a bound to start from).  At most BS_CHUNKS workgroups.
+void beam_chunks(int64_t rows, int64_t V, int* chunks, int* subs) {
+  const int n = (int)((V + BS_SUB - 1) / BS_SUB);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(BS_CHUNKS, (BS_WGS + rows - 1) / rows));
+  *subs = (int)((n + most - 1) / most);
   *chunks = (n + *subs - 1) / *subs;
 }
 
@@ -344,8 +378,12 @@ void beam_chunks(int V, int* chunks, int* subs) {
 
 extern "C" int64_t t2s_beam_select_workspace_bytes(int B, int N, int V, int n_select) {
   if (B <= 0 || N <= 0 || V <= 0 || n_select <= 0) return 0;
-  int chunks, subs;
-  beam_chunks(V, &chunks, &subs);
+  int chunks = 0, subs;
+  for (int skew : {0, 3, 7}) {                     // (more words may make fewer workgroups of more stretches)
+    int c;
+    beam_chunks((int64_t)B * N, (int64_t)V + skew, &c, &subs);
+    chunks = std::max(chunks, c);
+  }
   return (int64_t)B * N * chunks * (8 * (int64_t)n_select + 8 + 4);
 }
 
@@ -357,10 +395,13 @@ extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t
   T2S_CHECK_ARG(n_select > 0 && n_select <= BS_MAX && n_select <= (int64_t)N * V, "beam_select: %d of %d x %d candidates (at most %d)", n_select, N, V, BS_MAX);
   T2S_CHECK_ARG(pad >= 0 && pad < V, "beam_select: pad %d outside the vocabulary of %d", pad, V);
   T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "beam_select: bad dtype %d", dtype);
+  T2S_CHECK_ARG((uintptr_t)logits % (dtype == T2S_F32 ? 4 : 2) == 0, "beam_select: logits not aligned to their type");
   T2S_CHECK_ARG((uintptr_t)workspace % 8 == 0 && workspace_bytes >= t2s_beam_select_workspace_bytes(B, N, V, n_select), "beam_select: workspace of %lld bytes is too small",
                 (long long)workspace_bytes);
+  const int64_t es = dtype == T2S_F32 ? 4 : 2;
+  const bool whole = (uintptr_t)logits % 16 == 0 && batch_stride * es % 16 == 0 && beam_stride * es % 16 == 0;
   int chunks, subs;
-  beam_chunks(V, &chunks, &subs);
+  beam_chunks((int64_t)B * N, whole ? V : (int64_t)V + 16 / es - 1, &chunks, &subs);
   const int64_t rows = (int64_t)B * N, grid = rows * chunks;
   T2S_CHECK_ARG(grid < ((int64_t)1 << 31), "beam_select: too many rows");
   uint64_t* keys = (uint64_t*)workspace;

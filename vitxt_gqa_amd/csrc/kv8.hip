@@ -19,6 +19,7 @@
 // lane; the 16 bytes a lane loads of value row `dim` are then the A operand against exactly those tokens.  No LDS, no
 // shuffles between the two products, and every load of the pass is 16 contiguous bytes per lane.
 #include "common.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -32,9 +33,6 @@ constexpr float KV_LOG2E = 1.4426950408889634f;
 constexpr float KV_LN2 = 0.6931471805599453f;
 
 constexpr int FMT_INT8 = T2S_KV_INT8, FMT_E4M3 = T2S_KV_E4M3;
-
-__device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
-__device__ __forceinline__ uint32_t as_u(float f) { return __builtin_bit_cast(uint32_t, f); }
 
 // the block's scale from the bits of its largest magnitude (>= 0x7f800000: a value that is not finite -> NaN)
 template <int FMT>
@@ -109,59 +107,6 @@ __device__ __forceinline__ f16x8 decode8_f16(uint32_t lo, uint32_t hi) {
 
 // word position of token group tg (tokens 4 tg .. 4 tg + 3) inside a value row: p / 4 of the order above
 __device__ __forceinline__ int v_word(int tg) { return (tg & 3) * 4 + (tg >> 2); }
-
-// lane exchanges without LDS: the pairs (x[l], x[l ^ 16]) and (x[l], x[l ^ 32]) in some order
-__device__ __forceinline__ void swap16(float x, float& a, float& b) {
-  const auto p = __builtin_amdgcn_permlane16_swap(as_u(x), as_u(x), false, false);
-  a = as_f(p[0]);
-  b = as_f(p[1]);
-}
-__device__ __forceinline__ void swap32(float x, float& a, float& b) {
-  const auto p = __builtin_amdgcn_permlane32_swap(as_u(x), as_u(x), false, false);
-  a = as_f(p[0]);
-  b = as_f(p[1]);
-}
-// maximum / sum over the four 16-lane groups that hold one query's keys
-__device__ __forceinline__ float across_max(float x) {
-  float a, b;
-  swap16(x, a, b);
-  swap32(fmaxf(a, b), a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float across_sum(float x) {
-  float a, b;
-  swap16(x, a, b);
-  swap32(a + b, a, b);
-  return a + b;
-}
-// value of lane l ^ 1 / l ^ 2 (quad permutes), l + 4 / l + 8 in a ring of 16 (row rotations)
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return as_f((uint32_t)__builtin_amdgcn_mov_dpp((int)as_u(x), CTRL, 0xf, 0xf, true));
-}
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
-// maximum of an unsigned number over the wave
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  float a, b;
-  x = max(x, as_u(dpp<DPP_XOR1>(as_f(x))));
-  x = max(x, as_u(dpp<DPP_XOR2>(as_f(x))));
-  x = max(x, as_u(dpp<DPP_ROR4>(as_f(x))));
-  x = max(x, as_u(dpp<DPP_ROR8>(as_f(x))));
-  swap16(as_f(x), a, b);
-  swap32(as_f(max(as_u(a), as_u(b))), a, b);
-  return max(as_u(a), as_u(b));
-}
-// maximum / sum over the wave's sixteen quads, each of which holds one value four times
-__device__ __forceinline__ float quads_max(float x) {
-  x = fmaxf(x, dpp<DPP_ROR4>(x));
-  x = fmaxf(x, dpp<DPP_ROR8>(x));
-  return across_max(x);
-}
-__device__ __forceinline__ float quads_sum(float x) {
-  x += dpp<DPP_ROR4>(x);
-  x += dpp<DPP_ROR8>(x);
-  return across_sum(x);
-}
 
 // ------------------------------------------------------------------------------------------------------------------------------------
 // append.  One workgroup = one (sequence, head) walking the blocks that the new tokens touch; a thread owns 4 tokens x 4 dims of a block, of
