@@ -55,8 +55,9 @@ __device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v,
 
 // A bound that the K largest of a wave's 64 keys reach and, where keys are unique, no others do; 1 where fewer than K are not zero.  Two bits
 // at a time from the top, the lanes at or above the three trial values counted by ballots; done as soon as exactly K are left (some 10
-// steps on random logits, 32 at most)
-__device__ __forceinline__ uint64_t wave_kth(uint64_t key, int K) {
+// steps on random logits, 32 at most).  `least`: 1 as well where fewer than K are above it.
+__device__ __forceinline__ uint64_t wave_kth(uint64_t key, int K, uint64_t least) {
+  if (__popcll(__ballot(key > least)) < K) return 1;
   uint64_t t = 0;
   for (int bit = 62; bit >= 0; bit -= 2) {
     const uint64_t t1 = t | 1ull << bit, t2 = t | 2ull << bit, t3 = t | 3ull << bit;
@@ -64,7 +65,7 @@ __device__ __forceinline__ uint64_t wave_kth(uint64_t key, int K) {
     t = c3 >= K ? t3 : c2 >= K ? t2 : c1 >= K ? t1 : t;
     if (c1 == K || c2 == K || c3 == K) break;
   }
-  return t ? t : 1;
+  return t;
 }
 
 template <typename TX>
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
   __shared__ uint64_t list_s[4 * BS_MAX * (BS_EPT + 1)];
   __shared__ uint64_t top_s[BS_MAX];
   __shared__ uint32_t low_s[4];
-  __shared__ int cnt_s;
+  __shared__ int cnt_s, rank_s[64];
   __shared__ float m_s[4];
   __shared__ double s_s[4];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, chunk = blockIdx.x % chunks;
@@ -143,6 +144,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     const uint32_t low = max(wave_kth_bound(ordered(mx), K), (uint32_t)(top_s[K - 1] >> 32));
     if (lane == 0) low_s[wave] = low;
     if (tid == 0) cnt_s = 0;
+    if (tid < 64) rank_s[tid] = 0;
     __syncthreads();
     // (below -inf's form there is no number: everything passes)
     const uint32_t low4 = max(max(low_s[0], low_s[1]), max(low_s[2], low_s[3]));
@@ -159,7 +161,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     // of one key a lane, at most K (BS_EPT + 1); those are unique.
     uint64_t thr = 1;
     if (cnt > BS_LIST) {
-      thr = wave_kth(kept > best ? kept : best, K);
+      thr = wave_kth(kept > best ? kept : best, K, 0);
       cnt = __popcll(__ballot(kept >= thr));
       mask = 0;
 #pragma unroll
@@ -191,12 +193,23 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     for (int i = to + lane; i < end; i += 64) list_s[i] = 0;
     __syncthreads();
     const int total = cnt_s;
-    for (int i = tid; i < total; i += 256) {
-      const uint64_t mine = list_s[i];
+    if (total <= 64) {                             // a lane to a key, a quarter of the others to a wave
+      const uint64_t mine = lane < total ? list_s[lane] : 0;
+      const int each = (total + 3) >> 2, to_j = min(total, (wave + 1) * each);
       int rank = 0;
 #pragma unroll 8
-      for (int j = 0; j < total; ++j) rank += list_s[j] > mine;
-      if (rank < K) top_s[rank] = mine;                                  // (empty places rank behind all keys)
+      for (int j = wave * each; j < to_j; ++j) rank += list_s[j] > mine;
+      if (rank) atomicAdd(rank_s + lane, rank);
+      __syncthreads();
+      if (tid < total && rank_s[tid] < K) top_s[rank_s[tid]] = mine;     // (empty places rank behind all keys)
+    } else {
+      for (int i = tid; i < total; i += 256) {
+        const uint64_t mine = list_s[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < total; ++j) rank += list_s[j] > mine;
+        if (rank < K) top_s[rank] = mine;
+      }
     }
   }
   // ---- the row's maximum and sum over this workgroup
@@ -218,11 +231,12 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
   }
 }
 
+// A candidate in two integers: its score in an order-preserving form (0: no candidate), and ~(n << 32 | v), so that equal scores are in the
+// order of n V + v, lowest first, when the larger pair is the better one.
 struct __attribute__((aligned(16))) Cand {
-  double score;
-  int64_t flat;       // n << 32 | v, in the order of n V + v; INT64_MAX: no candidate
+  uint64_t score, place;
 };
-__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.flat < b.flat); }
+__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.score > b.score || (a.score == b.score && a.place > b.place); }
 
 constexpr int BJ_PER = 4;                          // candidates of a thread at a time
 
@@ -231,6 +245,7 @@ __device__ __forceinline__ uint64_t ordered64(double x) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
   return u >> 63 ? ~u : u | 1ull << 63;
 }
+__device__ __forceinline__ double from_ordered64(uint64_t k) { return __builtin_bit_cast(double, k >> 63 ? k ^ 1ull << 63 : ~k); }
 
 // one workgroup per sequence: joins the stretches, orders the N rows' candidates, 256 BJ_PER of them at a time
 __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restrict__ keys, const double* __restrict__ sums, const float* __restrict__ maxs,
@@ -240,11 +255,11 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
   __shared__ float top_m[BS_MAX], part_m[BS_MAX * BS_CHUNKS];
   __shared__ Cand list_s[256 * BJ_PER + BS_MAX], top_s[BS_MAX];
   __shared__ uint64_t thr_s[4];
-  __shared__ int cnt_s;
-  const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.x;
+  __shared__ int cnt_s, rank_s[64];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
   const int per_row = chunks * K, M = N * per_row;                     // (32 * 32 * 32 at most)
   const float per_inv = 1.0f / (float)per_row;
-  const Cand none{-INFINITY, INT64_MAX};
+  const Cand none{0, 0};
   const uint64_t* kb = keys + (int64_t)b * M;
   uint64_t raw[BJ_PER];                            // (in flight beside the rows' sums)
 #pragma unroll
@@ -274,7 +289,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
   for (int m0 = 0; m0 < M; m0 += 256 * BJ_PER) {
     Cand c[BJ_PER];
     const Cand kept = tid < K ? top_s[tid] : none;
-    uint64_t best = kept.flat != INT64_MAX ? ordered64(kept.score) : 0;
+    uint64_t best = kept.score;
 #pragma unroll
     for (int j = 0; j < BJ_PER; ++j) {
       const int i = m0 + tid + j * 256;
@@ -283,17 +298,19 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
       if (k) {
         const int n = (int)(((float)i + 0.5f) * per_inv);              // i / per_row: half a step from every border, 2^-23 relative off
         const float x = from_ordered((uint32_t)(k >> 32));
-        c[j].score = x > -INFINITY ? off_s[n] + ((double)x - (double)top_m[n]) : -INFINITY;
-        c[j].flat = (int64_t)n << 32 | (0xffffffffu - (uint32_t)k);
-        best = max(best, ordered64(c[j].score));
+        const double sc = x > -INFINITY ? off_s[n] + ((double)x - (double)top_m[n]) : -INFINITY;
+        c[j].score = ordered64(sc);
+        c[j].place = ~((uint64_t)n << 32 | (0xffffffffu - (uint32_t)k));
+        best = max(best, c[j].score);
       }
     }
     // a lower bound for the K-th best score, as in the rows' kernel; equal scores are all listed (the list holds everything there is)
     if (tid == 0) cnt_s = 0;
+    if (tid < 64) rank_s[tid] = 0;
     uint64_t thr = 1;
     if (M > 64) {
-      thr = wave_kth(best, K);
-      if (lane == 0) thr_s[tid >> 6] = thr;
+      thr = wave_kth(best, K, 0x000fffffffffffffull);          // (-inf's form: a wave of few numbers leaves the bound to the others)
+      if (lane == 0) thr_s[wave] = thr;
     }
     __syncthreads();
     if (M > 64)
@@ -301,26 +318,37 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
     if (best >= thr) {
 #pragma unroll
       for (int j = 0; j < BJ_PER; ++j)
-        if (c[j].flat != INT64_MAX && ordered64(c[j].score) >= thr) list_s[atomicAdd(&cnt_s, 1)] = c[j];
-      if (kept.flat != INT64_MAX && ordered64(kept.score) >= thr) list_s[atomicAdd(&cnt_s, 1)] = kept;
+        if (c[j].score >= thr) list_s[atomicAdd(&cnt_s, 1)] = c[j];
+      if (kept.score >= thr) list_s[atomicAdd(&cnt_s, 1)] = kept;
     }
     __syncthreads();
     const int cnt = cnt_s;
-    for (int i = tid; i < cnt; i += 256) {
-      const Cand mine = list_s[i];
+    if (cnt <= 64) {                               // a lane to a candidate, a quarter of the others to a wave
+      const Cand mine = lane < cnt ? list_s[lane] : none;
+      const int each = (cnt + 3) >> 2, to_j = min(cnt, (wave + 1) * each);
       int rank = 0;
+#pragma unroll 4
+      for (int j = wave * each; j < to_j; ++j) rank += before(list_s[j], mine);
+      if (rank) atomicAdd(rank_s + lane, rank);
+      __syncthreads();
+      if (tid < cnt && rank_s[tid] < K) top_s[rank_s[tid]] = mine;
+    } else {
+      for (int i = tid; i < cnt; i += 256) {
+        const Cand mine = list_s[i];
+        int rank = 0;
 #pragma unroll 8
-      for (int j = 0; j < cnt; ++j) rank += before(list_s[j], mine);
-      if (rank < K) top_s[rank] = mine;
+        for (int j = 0; j < cnt; ++j) rank += before(list_s[j], mine);
+        if (rank < K) top_s[rank] = mine;
+      }
     }
     __syncthreads();
   }
   if (tid < K) {
     const Cand r = top_s[tid];
     const int64_t at = (int64_t)b * K + tid;
-    out_scores[at] = (float)r.score;
-    out_parents[at] = r.flat >> 32;
-    out_tokens[at] = r.flat & 0xffffffff;
+    out_scores[at] = (float)from_ordered64(r.score);
+    out_parents[at] = (int64_t)(~r.place >> 32);
+    out_tokens[at] = (int64_t)(~r.place & 0xffffffffu);
   }
 }
 
