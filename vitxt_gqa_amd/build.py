@@ -14,10 +14,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -fno-slp-vectorize: under plain -O3 the SLP vectoriser packs adjacent scalar f32 multiplies / adds of the attention kernels
 # into v_pk_mul_f32 / v_pk_fma_f32, which issue slower beside MFMAs than the scalar forms (MI355X_MICROARCH.md, per-instruction
 # constants); measured on the attention backward: 6.10 -> 5.87 ms without dropout, 7.95 -> 7.76 ms with (B=8, same box)
-FLAGS = ["--offload-arch=gfx950", "-O3", "-fno-slp-vectorize", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
-# the decode operators are compiled without packed fp32 instructions: some of their forms have given wrong results on this card now and then
-NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-NO_PACKED_FP32_FILES = ("kv8.hip", "beam.hip")
+# -packed-fp32-ops: no packed fp32 instructions at all, also where the code has pairs of floats: some of their forms have given wrong results on
+# this card now and then, without an error.  The train step is 0.7 % faster without them (659.1 / 659.6 -> 654.3 / 655.2 ms, same box, in turn).
+FLAGS = ["--offload-arch=gfx950", "-O3", "-fno-slp-vectorize", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 OBJ = os.path.join(HERE, "build")
 
 
@@ -42,9 +42,7 @@ def _object(src):
 
 
 def _compile(src, verbose):
-    out = _object(src)
-    extra = NO_PACKED_FP32 if os.path.basename(src) in NO_PACKED_FP32_FILES else []
-    cmd = [HIPCC] + FLAGS + extra + ["-c", src, "-o", out]
+    cmd = [HIPCC] + FLAGS + ["-c", src, "-o", _object(src)]
     if verbose:
         print("[vitxt_gqa_amd.build]", " ".join(cmd), flush=True)
     subprocess.check_call(cmd)
