@@ -45,11 +45,11 @@ __device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v,
     for (int i = 0; i < VEC; i += 4) {
       const f32x4 f = Vec4<TX>::load(x + v + i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i + j] = clean(f[j]);
+      for (int j = 0; j < 4; ++j) o[i + j] = f[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = v + i >= 0 && v + i < V ? clean((float)x[v + i]) : -INFINITY;
+    for (int i = 0; i < VEC; ++i) o[i] = v + i >= 0 && v + i < V ? (float)x[v + i] : -INFINITY;
   }
 }
 
@@ -116,27 +116,26 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
 #pragma unroll
       for (int i = 0; i < BS_EPT; i += VEC) load_logits<TX, VEC>(x, v0 + i * 256 + tid * VEC, V, val + i);
     auto index = [&](int i) { return v0 + (i / VEC) * VEC * 256 + tid * VEC + i % VEC; };       // rises with i
-    float mx = -INFINITY;
-    int at = index(0) < 0 ? (int)-index(0) : 0;                          // (the first that is of the row)
+    // maximum and sum of this lane's logits; a NaN or +inf among the wave's shows as a NaN sum, and is taken out (`clean`) then and only then
+    float mx, mn, s;
+    for (int pass = 0;; ++pass) {
+      mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < BS_EPT; ++i)
-      if (val[i] > mx) {
-        mx = val[i];
-        at = i;
-      }
-    // index(at) where `at` is a run-time value: the elements of a lane are VEC apart from the next ones of 256 lanes
-    const int64_t v_at = v0 + (at / VEC) * VEC * 256 + tid * VEC + at % VEC;
-    uint64_t best = v_at < V ? key_of(mx, v_at) : 0;
-    if (mx > m) {
-      sum *= (double)__expf(m - mx);
-      m = mx;
-    }
-    if (m > -INFINITY) {
-      float s = 0.f;
+      for (int i = 0; i < BS_EPT; ++i) mx = fmaxf(mx, val[i]);
+      mn = fmaxf(m, mx);
+      const float mu = mn > -INFINITY ? mn : 0.f;
+      s = 0.f;
 #pragma unroll
-      for (int i = 0; i < BS_EPT; ++i) s += __expf(val[i] - m);
-      sum += (double)s;
+      for (int i = 0; i < BS_EPT; ++i) s += __expf(val[i] - mu);
+      if (pass || !__any(s != s)) break;
+#pragma unroll
+      for (int i = 0; i < BS_EPT; ++i) val[i] = clean(val[i]);
     }
+    if (mn > m) {
+      sum *= (double)__expf(m - mn);
+      m = mn;
+    }
+    sum += (double)s;
     // ---- the K best of (this stretch, what is kept of the former ones).  A number that K lanes' best logits reach bounds the K-th largest from
     // below; the largest such number of the four waves, or the K-th of what is kept already, leaves little more than K logits to rank.
     __syncthreads();
@@ -149,18 +148,26 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     // (below -inf's form there is no number: everything passes)
     const uint32_t low4 = max(max(low_s[0], low_s[1]), max(low_s[2], low_s[3]));
     const float tv = low4 > 0x7fffffu ? from_ordered(low4) : -INFINITY;
-    uint32_t mask = 0;                                                  // this lane's logits that reach it
-    int cnt = __popcll(__ballot(kept != 0));
+    uint32_t below = 0;                                                 // bit i: this lane's logit i does not reach it (the sign of the difference)
+    if (tv > -INFINITY)
 #pragma unroll
-    for (int i = 0; i < BS_EPT; ++i) {
-      const bool in = val[i] >= tv;
-      cnt += __popcll(__ballot(in));
-      mask |= in ? 1u << i : 0u;
-    }
+      for (int i = BS_EPT - 1; i >= 0; --i) below = __builtin_amdgcn_alignbit(below, as_u(val[i] - tv), 31);
+    uint32_t mask = ~below & ((1u << BS_EPT) - 1u);
+    int cnt = (int)wave_sum_u(__popc(mask)) + __popcll(__ballot(kept != 0));
     // Many of them (logits in an order that defeats the bound, equal ones, lanes without any): only those that reach the wave's K-th best
     // of one key a lane, at most K (BS_EPT + 1); those are unique.
     uint64_t thr = 1;
     if (cnt > BS_LIST) {
+      int at = index(0) < 0 ? (int)-index(0) : 0;                       // the lane's best: the first that is of the row, or a larger one
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < BS_EPT; ++i)
+        if (val[i] > top) {
+          top = val[i];
+          at = i;
+        }
+      const int64_t v_at = v0 + (at / VEC) * VEC * 256 + tid * VEC + at % VEC;
+      const uint64_t best = v_at < V ? key_of(top, v_at) : 0;
       thr = wave_kth(kept > best ? kept : best, K, 0);
       cnt = __popcll(__ballot(kept >= thr));
       mask = 0;

@@ -59,6 +59,17 @@ __device__ __forceinline__ float quads_sum(float x) {
   x += dpp<DPP_ROR8>(x);
   return across_sum(x);
 }
+// sum of an unsigned number over the wave
+__device__ __forceinline__ uint32_t wave_sum_u(uint32_t x) {
+  float a, b;
+  x += as_u(dpp<DPP_XOR1>(as_f(x)));
+  x += as_u(dpp<DPP_XOR2>(as_f(x)));
+  x += as_u(dpp<DPP_ROR4>(as_f(x)));
+  x += as_u(dpp<DPP_ROR8>(as_f(x)));
+  swap16(as_f(x), a, b);
+  swap32(as_f(as_u(a) + as_u(b)), a, b);
+  return __builtin_amdgcn_readfirstlane(as_u(a) + as_u(b));
+}
 // maximum over the wave (NaN counts as nothing)
 __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, dpp<DPP_XOR1>(x));
