@@ -19,6 +19,9 @@
 
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int BS_MAX = T2S_BEAM_MAX;               // beams, and candidates to select
 constexpr int BS_EPT = 16;                         // elements of a thread per stretch
 constexpr int BS_SUB = 256 * BS_EPT;
@@ -368,22 +371,18 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(U* __restrict__ state
   const int b = blockIdx.y;
   if (u >= used_units) return;
   U* base = state + ((int64_t)blockIdx.z * B + b) * N * row_units + u;
-  const int64_t* pb = parents + (int64_t)b * N;
+  int from[NT];                                    // the beam a beam comes from; itself where it stays (or is none)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int64_t p = n < N ? parents[(int64_t)b * N + n] : n;
+    from[n] = n >= N ? n : (int)(p < 0 ? 0 : (p >= N ? N - 1 : p));
+  }
   U val[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-    if (n < N) {
-      int64_t p = pb[n];
-      p = p < 0 ? 0 : (p >= N ? N - 1 : p);
-      if (p != n) val[n] = base[p * row_units];
-    }
+  for (int n = 0; n < NT; ++n) val[n] = from[n] != n ? base[from[n] * row_units] : U{};
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-    if (n < N) {
-      int64_t p = pb[n];
-      p = p < 0 ? 0 : (p >= N ? N - 1 : p);
-      if (p != n) base[n * row_units] = val[n];
-    }
+    if (from[n] != n) base[n * row_units] = val[n];
 }
 
 template <typename U>
@@ -461,8 +460,8 @@ extern "C" int t2s_beam_reorder(void* state, const int64_t* parents, int outer, 
   T2S_CHECK_ARG(used_bytes > 0 && used_bytes <= row_bytes, "beam_reorder: %lld of %lld bytes", (long long)used_bytes, (long long)row_bytes);
   hipStream_t st = (hipStream_t)stream;
   const uint64_t al = (uint64_t)(uintptr_t)state | (uint64_t)row_bytes | (uint64_t)used_bytes;
-  if (al % 16 == 0) return launch_reorder<uint4>(state, parents, outer, B, N, row_bytes, used_bytes, st);
-  if (al % 8 == 0) return launch_reorder<uint2>(state, parents, outer, B, N, row_bytes, used_bytes, st);
+  if (al % 16 == 0) return launch_reorder<u32x4>(state, parents, outer, B, N, row_bytes, used_bytes, st);
+  if (al % 8 == 0) return launch_reorder<u32x2>(state, parents, outer, B, N, row_bytes, used_bytes, st);
   if (al % 4 == 0) return launch_reorder<uint32_t>(state, parents, outer, B, N, row_bytes, used_bytes, st);
   if (al % 2 == 0) return launch_reorder<uint16_t>(state, parents, outer, B, N, row_bytes, used_bytes, st);
   return launch_reorder<uint8_t>(state, parents, outer, B, N, row_bytes, used_bytes, st);
