@@ -23,6 +23,7 @@ BLOCK = 64                  # tokens of a block: one scale for its keys and one 
 HEAD_DIM = 64
 BEAM_MAX = X.T2S_BEAM_MAX   # beams, and candidates a selection returns
 FORMATS = {"int8": (X.T2S_KV_INT8, torch.int8), "e4m3": (X.T2S_KV_E4M3, torch.float8_e4m3fn)}
+_empty = torch.empty_strided         # (of torch's ways to allocate the one with the least overhead: it counts in calls that take a few microseconds)
 _DTYPES = {torch.float32: (X.T2S_F32, 15), torch.bfloat16: (X.T2S_BF16, 7)}          # code, mask of a 4-element alignment in bytes
 
 
@@ -51,16 +52,17 @@ def _launch(index, fn, *args):
 
 
 def _head_rows(t, name):
-    """Strides of [..., heads, 64] with dense 64-element rows that start at multiples of 4 elements (0 for axes of length 1)."""
+    """Strides of [..., heads, 64] with dense 64-element rows that start at multiples of 4 elements (0 for axes of length 1), and its address."""
     s = t.stride()
     d = _DTYPES.get(t.dtype)
-    if d is None or t.shape[-1] != HEAD_DIM or s[-1] != 1 or t.data_ptr() & d[1] or any([x & 3 for x in s[:-1]]):
+    at = t.data_ptr()
+    if d is None or s[-1] != 1 or t.shape[-1] != HEAD_DIM or at & d[1] or (s[0] | s[1] | s[2] | (s[3] if len(s) == 5 else 0)) & 3:
         _need(d is not None, "%s: float32 or bfloat16, got %s", name, t.dtype)
         _need(t.shape[-1] == HEAD_DIM, "%s: the kernels are built for head_dim 64, got %s", name, tuple(t.shape))
         s = tuple(x if n > 1 else 0 for x, n in zip(s[:-1], t.shape[:-1])) + (s[-1],)
-        _need(s[-1] == 1 and not t.data_ptr() & d[1] and not any(x & 3 for x in s[:-1]),
+        _need(s[-1] == 1 and not at & d[1] and not any(x & 3 for x in s[:-1]),
               "%s: rows of 64 dense elements, aligned to 4 elements, are needed (strides %s): call .contiguous()", name, t.stride())
-    return s
+    return s, at
 
 
 @functools.lru_cache(maxsize=256)
@@ -148,11 +150,11 @@ class KVCache8:
         elif T > self.capacity:
             _need(False, "append: %d tokens do not fit a capacity of %d", T, self.capacity)
         _need(R > 0 or T == 0, "append: %d tokens of no rows", T)
-        sk, sv = (_head_rows(k, "append: k"), _head_rows(v, "append: v")) if T else (None, None)
+        (sk, kp), (sv, vp) = (_head_rows(k, "append: k"), _head_rows(v, "append: v")) if T else ((None, None),) * 2
         _same_device(self._index, k, v, counts, rows)
         if T == 0:
             return self
-        X.check(_launch(self._index, X.lib().t2s_kv8_append, k.data_ptr(), sk[0], sk[1], sk[2], v.data_ptr(), sv[0], sv[1], sv[2], rp, rs, cp, *self._ptrs,
+        X.check(_launch(self._index, X.lib().t2s_kv8_append, kp, sk[0], sk[1], sk[2], vp, sv[0], sv[1], sv[2], rp, rs, cp, *self._ptrs,
                         self._ticket_ptr, B, H, T, R, self.blocks, _DTYPES[k.dtype][0], self._fmt), "t2s_kv8_append")
         self.max_len = min(self.capacity, self.max_len + T)
         return self
@@ -176,7 +178,9 @@ class KVCache8:
         """(keys, values) [B, H, capacity, 64] in ``dtype`` (float32 or bfloat16): code * scale, zeros behind a sequence's length."""
         _need(dtype in (torch.bfloat16, torch.float32), "dequantize: float32 or bfloat16, got %s", dtype)
         _same_device(self._index, self.k)
-        k, v = (torch.empty(self.batch, self.heads, self.capacity, HEAD_DIM, dtype=dtype, device=self.device) for _ in range(2))
+        shape, n = (self.batch, self.heads, self.capacity, HEAD_DIM), self.capacity * HEAD_DIM
+        strides = (self.heads * n, n, HEAD_DIM, 1)
+        k, v = _empty(shape, strides, dtype=dtype, device=self.device), _empty(shape, strides, dtype=dtype, device=self.device)
         X.check(_launch(self._index, X.lib().t2s_kv8_dequantize, *self._ptrs, k.data_ptr(), v.data_ptr(), self.batch, self.heads, self.blocks,
                         _DTYPES[dtype][0], self._fmt), "t2s_kv8_dequantize")
         return k, v
@@ -197,7 +201,7 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
     if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[2] < 1 or q.shape[2] % H:
         _need(False, "attend: q [%d, N, a multiple of %d, 64], got %s", cache.batch, H, tuple(q.shape))
     B, N, HQ, _ = q.shape
-    sq = _head_rows(q, "attend: q")
+    sq, qp = _head_rows(q, "attend: q")
     T, tk, tv, st, tl, tls = 0, None, None, (0, 0, 0, 0), None, (0, 0)
     if tail_k is not None and tail_v is not None:
         T = tail_k.shape[2] if tail_k.dim() == 5 else -1
@@ -209,22 +213,24 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
         elif tail_len is not None:
             T = max(0, min(int(tail_len), T))
         if T > 0:
-            st = _head_rows(tail_k, "attend: tail_k")
-            if _head_rows(tail_v, "attend: tail_v") != st:
+            st, tk = _head_rows(tail_k, "attend: tail_k")
+            sv, tv = _head_rows(tail_v, "attend: tail_v")
+            if sv != st:
                 _need(False, "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
-            tk, tv = tail_k.data_ptr(), tail_v.data_ptr()
     else:
         _need(tail_k is None and tail_v is None, "attend: tail_k and tail_v come together")
         _need(tail_len is None, "attend: tail_len without a tail")
     _same_device(cache._index, q, tail_k, tail_v, None if tl is None else tail_len)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, N, HQ), dtype=torch.float32, device=q.device)
+    dev, n = q.device, HQ * HEAD_DIM
+    out = _empty((B, N, HQ, HEAD_DIM), (N * n, n, HEAD_DIM, 1), dtype=q.dtype, device=dev)
+    lse = _empty((B, N, HQ), (N * HQ, HQ, 1), dtype=torch.float32, device=dev)
     if N == 0:
         return out, lse
-    splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len, _DTYPES[q.dtype][0])
-    ws = torch.empty(nbytes // 4, dtype=torch.float32, device=q.device) if nbytes else None
-    X.check(_launch(cache._index, X.lib().t2s_kv8_attn, q.data_ptr(), sq[0], sq[1], sq[2], *cache._ptrs, tk, tv, st[0], st[1], st[2], st[3], tl, tls[0], tls[1], T,
-                    out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, _DTYPES[q.dtype][0], cache._fmt), "t2s_kv8_attn")
+    code = _DTYPES[q.dtype][0]
+    splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len, code)
+    ws = _empty((nbytes // 4,), (1,), dtype=torch.float32, device=dev) if nbytes else None
+    X.check(_launch(cache._index, X.lib().t2s_kv8_attn, qp, sq[0], sq[1], sq[2], *cache._ptrs, tk, tv, st[0], st[1], st[2], st[3], tl, tls[0], tls[1], T,
+                    out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, code, cache._fmt), "t2s_kv8_attn")
     return out, lse
 
 
@@ -256,14 +262,16 @@ def beam_select(logits, scores, n_select, finished=None, pad=0):
         fp = finished.data_ptr()
     index = logits.get_device()
     _same_device(index, logits, scores, finished)
-    out = torch.empty((B, K), dtype=torch.float32, device=logits.device)
-    parents, tokens = torch.empty((2, B, K), dtype=torch.int64, device=logits.device).unbind(0)
+    dev = logits.device
+    out = _empty((B, K), (K, 1), dtype=torch.float32, device=dev)
+    parents, tokens = _empty((B, K), (K, 1), dtype=torch.int64, device=dev), _empty((B, K), (K, 1), dtype=torch.int64, device=dev)
     if B == 0:
         return out, parents, tokens
     scores = scores.contiguous()
     nbytes = _select_bytes(B, N, V, K)
-    ws = torch.empty((nbytes + 7) // 8, dtype=torch.int64, device=logits.device)
-    X.check(_launch(index, X.lib().t2s_beam_select, logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(), fp, pad, out.data_ptr(), parents.data_ptr(),
+    ws = _empty(((nbytes + 7) // 8,), (1,), dtype=torch.int64, device=dev)
+    sb, sn = logits.stride()[:2]
+    X.check(_launch(index, X.lib().t2s_beam_select, logits.data_ptr(), sb, sn, scores.data_ptr(), fp, pad, out.data_ptr(), parents.data_ptr(),
                     tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, d[0]), "t2s_beam_select")
     return out, parents, tokens
 
