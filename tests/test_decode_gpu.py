@@ -403,6 +403,18 @@ def test_select_ties_go_to_the_lowest_index():
     assert t.tolist() == [[0, 1, 2, 3, 4]]
 
 
+def test_select_negative_zeros_on_top():
+    """Rows whose best logits are -0.0: the same number as 0, and not below a bound of it."""
+    for V in (4096, 9001):
+        for dtype in (torch.float32, torch.bfloat16):
+            x = torch.full((2, 2, V), -3.0, dtype=dtype)
+            x[:, :, 5::16] = -0.0
+            _, _, t = _check_select(x, torch.tensor([[0.0, -9.0]] * 2), 7)
+            assert t.tolist() == [list(range(5, 5 + 7 * 16, 16))] * 2
+            _, _, t = _check_select(torch.full((1, 1, V), -0.0, dtype=dtype), torch.zeros(1, 1), 32)
+            assert t.tolist() == [list(range(32))]
+
+
 def test_select_first_step_and_dead_beams():
     g = torch.Generator().manual_seed(32)
     logits = torch.randn(2, 5, 700, generator=g)

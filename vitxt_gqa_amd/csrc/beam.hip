@@ -150,7 +150,8 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     __syncthreads();
     // (below -inf's form there is no number: everything passes)
     const uint32_t low4 = max(max(low_s[0], low_s[1]), max(low_s[2], low_s[3]));
-    const float tv = low4 > 0x7fffffu ? from_ordered(low4) : -INFINITY;
+    // (a bound of zero as -0: x - -0 has the sign bit of neither zero, -0 - 0 would have it)
+    const float tv = low4 == 0x80000000u ? -0.0f : low4 > 0x7fffffu ? from_ordered(low4) : -INFINITY;
     uint32_t below = 0;                                                 // bit i: this lane's logit i does not reach it (the sign of the difference)
     if (tv > -INFINITY)
 #pragma unroll
