@@ -30,6 +30,24 @@ def test_cache_shapes():
     assert c.set_lens(torch.tensor([3, 9], dtype=torch.int32)).lens.tolist() == [3, 9]
 
 
+def test_cache_storage_is_its_own():
+    """The storage of a cache stays what it was made with; copies have addresses of their own."""
+    import copy
+    import io
+    c = _cache().set_lens(5)
+    with pytest.raises(AttributeError):
+        c.k = torch.zeros_like(c.k)
+    with pytest.raises(AttributeError):
+        c.lens = torch.zeros_like(c.lens)
+    buf = io.BytesIO()
+    torch.save(c, buf)
+    buf.seek(0)
+    for d, own in ((copy.deepcopy(c), True), (torch.load(buf, weights_only=False), True), (copy.copy(c), False)):
+        assert d._ptrs == tuple(t.data_ptr() for t in (d.k, d.v, d.k_scale, d.v_scale, d.lens)) and d._ticket_ptr == d._ticket.data_ptr() != c._ticket_ptr
+        assert (d.k.data_ptr() != c.k.data_ptr()) == own and d.lens.tolist() == [5, 5] and (d.max_len, d.fmt, d.capacity) == (5, "int8", 128)
+    assert decode.KVCache8.from_parts(c.k, c.v, c.k_scale, c.v_scale, c.lens, -3).max_len == 0
+
+
 @pytest.mark.parametrize("make", [
     lambda c: decode.KVCache8(2, 3, 64, "int4", device="cpu"),
     lambda c: decode.KVCache8(0, 3, 64, device="cpu"),

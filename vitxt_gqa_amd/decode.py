@@ -119,12 +119,19 @@ class KVCache8:
             _need(t.is_contiguous(), "KVCache8: the storage has to be contiguous")
             _need(t.device == k.device, "KVCache8: the storage has to live on one device")
         self.fmt, self._fmt = fmt[0], FORMATS[fmt[0]][0]
-        self.k, self.v, self.k_scale, self.v_scale, self.lens = k, v, ks, vs, lens
+        self._parts = (k, v, ks, vs, lens)
         self.batch, self.heads, self.blocks, self.capacity, self.device = B, H, n, n * BLOCK, k.device
-        self.max_len = self.capacity if max_len is None else min(int(max_len), self.capacity)
+        self.max_len = self.capacity if max_len is None else max(0, min(int(max_len), self.capacity))
         self._ticket = torch.zeros(B, dtype=torch.int32, device=k.device)
         self._index = k.get_device()
-        self._ptrs, self._ticket_ptr = tuple(t.data_ptr() for t in (k, v, ks, vs, lens)), self._ticket.data_ptr()
+        self._ptrs, self._ticket_ptr = tuple(t.data_ptr() for t in self._parts), self._ticket.data_ptr()
+
+    # (the storage is fixed for the cache's life: its addresses are taken once)
+    k, v, k_scale, v_scale, lens = (property(lambda self, i=i: self._parts[i]) for i in range(5))
+
+    def __reduce__(self):
+        """Copies and pickles are caches of their own storage (``copy.copy``: another handle on the same)."""
+        return KVCache8.from_parts, (*self._parts, self.max_len)
 
     def append(self, k, v, counts=None, rows=None):
         """Puts new tokens behind what each sequence holds.  k, v: [B, R, H, 64] float32 or bfloat16, dense 64-element rows (slices of a fused
