@@ -262,6 +262,18 @@ def test_attend_views():
         _check_attend(_rows(g, B, H, N, HD, dtype=dt).cuda().transpose(1, 2), cache)
 
 
+def test_attend_tails_of_one_token_differ_in_strides_that_do_not_count():
+    g = torch.Generator().manual_seed(24)
+    cache = _filled(g, 1, 2, [100])
+    k, v = _rows(g, 1, 3, 5, 2, HD).cuda(), _rows(g, 1, 3, 1, 2, HD).cuda()
+    wide = torch.zeros(1, 3, 2, HD + 4, device="cuda")[..., :HD].unsqueeze(2)                   # odd steps of the axis of length 1
+    for tk, tv in ((k[:, :, :1].contiguous(), v), (v.clone(), v.as_strided(v.shape, (999, *v.stride()[1:2], 7, *v.stride()[3:])))):
+        _check_attend(_rows(g, 1, 3, 2, HD).cuda(), cache, tk, tv)
+    from vitxt_gqa_amd import decode
+    with pytest.raises(ValueError, match="same strides"):
+        decode.attend(_rows(g, 1, 3, 2, HD).cuda(), cache, v, wide)
+
+
 def test_attend_peaky_scores():
     """Scores of hundreds of nats, rising and falling along the cache: the running maximum moves at every block, late and early ones dominate."""
     from vitxt_gqa_amd import decode

@@ -223,7 +223,7 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
             st, tk = _head_rows(tail_k, "attend: tail_k")
             sv, tv = _head_rows(tail_v, "attend: tail_v")
             if sv != st:
-                _need(False, "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
+                _need(all(a == b or n == 1 for a, b, n in zip(sv, st, tail_k.shape)), "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
     else:
         _need(tail_k is None and tail_v is None, "attend: tail_k and tail_v come together")
         _need(tail_len is None, "attend: tail_len without a tail")
