@@ -147,6 +147,18 @@ def test_c_abi_refuses(lib):
     assert lib.t2s_beam_reorder(p, p, 1, 1, 3, 16, 32, None) != 0 and b"bytes" in lib.t2s_last_error()
     assert lib.t2s_kv8_attn_splits(0, 1, 1, 1, 64, 0) == 0 and lib.t2s_kv8_attn_splits(1, 1, 1, 1, 0, 1) == 1
     assert lib.t2s_beam_select_workspace_bytes(0, 1, 1, 1) == 0
+    # shapes whose products pass 32 bits are refused, none ends the process
+    big = 2 ** 31 - 1
+    assert lib.t2s_kv8_attn_splits(1, 65536, 1, 65536, 64, 0) == 0 and lib.t2s_kv8_attn_splits(big, 1, big, 1, 64, 0) == 0 and lib.t2s_kv8_attn_splits(1, 1, 1, 1, big, 0) > 1
+    assert lib.t2s_kv8_attn_workspace_bytes(1, 65536, 1, 65536, 2) == 0 and lib.t2s_kv8_attn_workspace_bytes(1, 1, 1, 1, 0) == 0
+    for n, h, grp in ((65536, 1, 65536), (big, big, 1), (4097, 4096, 1)):
+        a = list(att)
+        a[25], a[26], a[27] = n, h, grp
+        assert lib.t2s_kv8_attn(*a) != 0 and b"bad shape" in lib.t2s_last_error()
+    a = list(sel)
+    a[10:13] = big, 1 << 24, 3
+    assert lib.t2s_beam_select(*a) != 0 and (b"too many rows" in lib.t2s_last_error() or b"too small" in lib.t2s_last_error())
+    assert lib.t2s_beam_reorder(p, p, 1, 1, 3, 1 << 40, 1 << 40, None) != 0 and b"too long" in lib.t2s_last_error()
 
 
 def test_reference_statements():

@@ -390,7 +390,7 @@ template <typename U>
 int launch_reorder(void* state, const int64_t* parents, int outer, int B, int N, int64_t row_bytes, int64_t used_bytes, hipStream_t st) {
   const int64_t ru = row_bytes / (int64_t)sizeof(U), uu = used_bytes / (int64_t)sizeof(U);
   const int64_t gx = (uu + 255) / 256;
-  T2S_CHECK_ARG(gx < ((int64_t)1 << 31), "beam_reorder: rows too long");
+  T2S_CHECK_ARG(gx < ((int64_t)1 << 24), "beam_reorder: rows too long");
   dim3 grid((unsigned)gx, (unsigned)B, (unsigned)outer), block(256);
   if (N <= 4) hipLaunchKernelGGL((beam_reorder_kernel<U, 4>), grid, block, 0, st, (U*)state, parents, B, N, ru, uu);
   else if (N <= 8) hipLaunchKernelGGL((beam_reorder_kernel<U, 8>), grid, block, 0, st, (U*)state, parents, B, N, ru, uu);
@@ -438,7 +438,7 @@ extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t
   int chunks, subs;
   beam_chunks((int64_t)B * N, whole ? V : (int64_t)V + 16 / es - 1, &chunks, &subs);
   const int64_t rows = (int64_t)B * N, grid = rows * chunks;
-  T2S_CHECK_ARG(grid < ((int64_t)1 << 31), "beam_select: too many rows");
+  T2S_CHECK_ARG(grid < ((int64_t)1 << 24), "beam_select: too many rows");
   uint64_t* keys = (uint64_t*)workspace;
   double* sums = (double*)(keys + grid * n_select);
   float* maxs = (float*)(sums + grid);

@@ -769,6 +769,13 @@ constexpr int DEQUANTIZE_WGS = 40960;
 
 bool kv8_bad_fmt(int fmt) { return fmt != FMT_INT8 && fmt != FMT_E4M3; }
 
+// what a grid axis of 256 threads a workgroup can count: pairs, and output rows (a join may take a workgroup to a row)
+bool kv8_attn_shape(int B, int N, int H, int G) {
+  constexpr int64_t most = (int64_t)1 << 24;
+  if (B <= 0 || N <= 0 || H <= 0 || G <= 0 || (int64_t)B * H >= most || (int64_t)N * G >= most) return false;
+  return (int64_t)B * H * ((int64_t)N * G) < most;
+}
+
 // Row groups of a (sequence, head), each of which reads its cache: as few as registers allow (64 rows; fp32, with three terms to everything,
 // 32), of equal size; returns the 16-row tiles of a group.
 int attn_row_tiles(int rows, int dtype, int* groups) {
@@ -836,8 +843,8 @@ extern "C" int t2s_kv8_dequantize(const void* k8, const void* v8, const float* k
 }
 
 extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens, int dtype) {
-  if (B <= 0 || N <= 0 || H <= 0 || G <= 0) return 0;
-  const int blocks = max_tokens > 0 ? (max_tokens + KV_BLOCK - 1) / KV_BLOCK : 1;
+  if (!kv8_attn_shape(B, N, H, G)) return 0;
+  const int blocks = max_tokens > 0 ? (int)(((int64_t)max_tokens + KV_BLOCK - 1) / KV_BLOCK) : 1;
   int groups;
   attn_row_tiles(N * G, dtype, &groups);
   const int64_t pairs = (int64_t)B * H * groups;
@@ -849,6 +856,7 @@ extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens, i
 }
 
 extern "C" int64_t t2s_kv8_attn_workspace_bytes(int B, int N, int H, int G, int splits) {
+  if (!kv8_attn_shape(B, N, H, G) || splits < 1) return 0;
   return splits > 1 || N * G > DIRECT_ROWS ? (int64_t)B * H * (splits + 1) * N * G * (KV_HD + 2) * 4 : 0;
 }
 
@@ -859,7 +867,7 @@ extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row
                             void* workspace, int64_t workspace_bytes, int splits, int B, int N, int H, int G, int nblk, float scale, int dtype,
                             int fmt, t2s_stream_t stream) {
   T2S_CHECK_ARG(q && k8 && v8 && k_scale && v_scale && lens && out && lse && (workspace || !workspace_bytes), "kv8_attn: null pointer");
-  T2S_CHECK_ARG(B > 0 && N > 0 && H > 0 && G > 0 && nblk > 0 && nblk < (1 << 25) && (int64_t)N * G < (1 << 24) && (int64_t)B * H < (1 << 24),
+  T2S_CHECK_ARG(kv8_attn_shape(B, N, H, G) && nblk > 0 && nblk < (1 << 25),
                 "kv8_attn: bad shape B=%d N=%d H=%d G=%d nblk=%d", B, N, H, G, nblk);
   T2S_CHECK_ARG(dtype == T2S_F32 || dtype == T2S_BF16, "kv8_attn: bad dtype %d", dtype);
   T2S_CHECK_ARG(!kv8_bad_fmt(fmt), "kv8_attn: bad format %d", fmt);
@@ -884,7 +892,7 @@ extern "C" int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row
   a.row_tiles = groups;
   a.part_o = (float*)workspace;
   a.part_ml = a.part_o + (int64_t)B * H * a.nshare * rows * KV_HD;
-  T2S_CHECK_ARG(a.row_tiles <= 65535 && splits <= 65000 && (int64_t)B * H * rows < ((int64_t)1 << 31), "kv8_attn: too many rows or shares");
+  T2S_CHECK_ARG(a.row_tiles <= 65535 && splits <= 65000, "kv8_attn: too many rows or shares");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == T2S_BF16) {
     if (fmt == FMT_INT8) launch_attn<bf16_t, FMT_INT8>(a, qt, st);
