@@ -262,6 +262,59 @@ def test_attend_views():
         _check_attend(_rows(g, B, H, N, HD, dtype=dt).cuda().transpose(1, 2), cache)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("lens,N,H,G,T", [
+    ([300, 65], 40, 1, 1, 3), ([640, 1], 1, 1, 48, 20), ([200], 8, 2, 8, 0), ([129], 64, 1, 1, 33), ([500, 0], 65, 1, 1, 2), ([70], 9, 1, 16, 16), ([1500], 6, 1, 5, 0), ([40], 2, 1, 4, 17),
+    ([40], 3, 1, 3, 17), ([1400], 43, 1, 3, 1)])
+def test_attend_row_groups(dtype, lens, N, H, G, T):
+    """One to four 16-row tiles to a group and several groups, with a short cache (a single share) and a longer one, tails on either side of
+    what a single share takes in."""
+    g = torch.Generator().manual_seed(sum(lens) + N * 7 + G)
+    cache = _filled(g, len(lens), H, lens, "int8" if N % 2 else "e4m3")
+    q = (_rows(g, len(lens), N, H * G, HD) * 2).to(DT[dtype]).cuda()
+    tk = tv = tl = None
+    if T:
+        tk, tv = (_rows(g, len(lens), N, T, H, HD, dtype=DT[dtype]).cuda() for _ in range(2))
+        tl = torch.randint(0, T + 1, (len(lens), N), generator=g, dtype=torch.int32)
+    _check_attend(q, cache, tk, tv, tl)
+
+
+def test_attend_rows_do_not_touch_each_other():
+    """A row of NaN or infinite queries, or with a NaN in its tail, leaves the other rows of its tile as they were."""
+    from vitxt_gqa_amd import decode
+    g = torch.Generator().manual_seed(25)
+    cache = _filled(g, 1, 2, [333])
+    for dt in (torch.float32, torch.bfloat16):
+        q = _rows(g, 1, 7, 4, HD, dtype=dt).cuda()
+        tk, tv = (_rows(g, 1, 7, 6, 2, HD, dtype=dt).cuda() for _ in range(2))
+        a, la = decode.attend(q, cache, tk, tv)
+        q2, tk2, tv2 = q.clone(), tk.clone(), tv.clone()
+        q2[0, 1] = math.nan
+        q2[0, 3, 2, 5] = math.inf
+        tv2[0, 4, 2, 1, 9] = math.nan
+        tk2[0, 5, 5] = math.nan
+        b, lb = decode.attend(q2, cache, tk2, tv2, 5)
+        c, lc = decode.attend(q, cache, tk, tv, 5)
+        bad = torch.zeros(1, 7, 4, HD, dtype=torch.bool)
+        bad[0, 1] = bad[0, 3, 2] = True
+        bad[0, 4, 2:, 9] = True
+        bad = bad.cuda()
+        assert bool(torch.isnan(b[bad]).all()) and torch.equal(b[~bad], c[~bad])
+        _check_attend(q, cache, tk, tv, got=(a, la))
+        _check_attend(q, cache, tk, tv, torch.full((1, 7), 5, dtype=torch.int32), got=(c, lc))
+
+
+def test_attend_overflowing_scores_show():
+    """Scores past fp32's range have no softmax in fp32: NaN, not a number made of the others."""
+    from vitxt_gqa_amd import decode
+    cache = decode.KVCache8(1, 1, 200)
+    cache.append(torch.full((1, 200, 1, HD), 1e30).cuda(), torch.ones(1, 200, 1, HD).cuda())
+    for dt in (torch.float32, torch.bfloat16):
+        for N in (1, 12):
+            out, lse = decode.attend(torch.full((1, N, 1, HD), 1e20, dtype=dt).cuda(), cache)
+            assert bool(torch.isnan(out).all()) and not bool(torch.isfinite(lse).any())
+
+
 def test_attend_tails_of_one_token_differ_in_strides_that_do_not_count():
     g = torch.Generator().manual_seed(24)
     cache = _filled(g, 1, 2, [100])
@@ -425,6 +478,67 @@ def test_select_negative_zeros_on_top():
             assert t.tolist() == [list(range(5, 5 + 7 * 16, 16))] * 2
             _, _, t = _check_select(torch.full((1, 1, V), -0.0, dtype=dtype), torch.zeros(1, 1), 32)
             assert t.tolist() == [list(range(32))]
+
+
+@pytest.mark.parametrize("order", ["up", "down", "lanes", "stretches", "few", "steps"])
+def test_select_in_orders_that_defeat_the_bound(order):
+    """Orders in which a lane's or a wave's best says little of the others: rising, falling, the best in one lane, in one stretch, almost all masked, few values."""
+    g = torch.Generator().manual_seed(36)
+    for V, N, K in ((4096, 2, 32), (9000, 3, 32), (30000, 2, 5), (70001, 1, 32)):
+        x = torch.sort(torch.randn(2, N, V, generator=g) * 3, -1).values
+        at = torch.arange(V)
+        if order == "down":
+            x = x.flip(-1)
+        elif order == "lanes":                                  # the largest logits 1 024 elements apart
+            to = torch.argsort(at % 1024, stable=True)
+            x = torch.empty_like(x).index_copy_(2, to, x.flip(-1))
+        elif order == "stretches":
+            x = x.roll(V // 2 + 17, -1)
+        elif order == "few":
+            x = torch.where(torch.rand(2, N, V, generator=g) < 20.0 / V, x, torch.full_like(x, -math.inf))
+        elif order == "steps":
+            x = (x * 2).round() / 2
+        s = -torch.rand(2, N, generator=g)
+        for dt in (torch.float32, torch.bfloat16):
+            _check_select_ordered(x.to(dt), s, K)
+            _check_select_ordered(x.to(dt), torch.zeros(2, N), K)
+
+
+def _check_select_ordered(x, s, K):
+    """The statement's order wherever its scores differ clearly; equal logits of a row in the order of their places."""
+    from vitxt_gqa_amd import decode
+    got, p, t = (r.cpu() for r in decode.beam_select(x.cuda(), s.cuda(), K))
+    best, rp, rt = select_ref(x, s, K)
+    ref = best[:, :K]
+    inf = ref == -math.inf
+    assert torch.equal(got.double() == -math.inf, inf) and bool(((got.double() - ref).abs() <= 160 * U + U * ref.abs())[~inf].all())
+    total = (s.double()[..., None] + torch.log_softmax(x.double(), -1)).flatten(1)
+    V = x.shape[2]
+    for b in range(x.shape[0]):
+        picked = (p[b] * V + t[b]).tolist()
+        assert len(set(picked)) == K and all(0 <= w < V for w in t[b].tolist())
+        mine = total[b, picked]
+        assert bool(((mine - ref[b])[~inf[b]].abs() <= 2 * 160 * U).all())         # a permutation among scores that are equal up to the tolerance at most
+        for i in range(1, K):
+            if p[b, i] == p[b, i - 1] and x[b, p[b, i], t[b, i]] == x[b, p[b, i], t[b, i - 1]]:
+                assert t[b, i] > t[b, i - 1]
+
+
+def test_select_rows_that_start_anywhere():
+    """Many rows (several stretches to a workgroup) and lengths around a stretch, at every offset of a 16-byte unit."""
+    from vitxt_gqa_amd import decode
+    g = torch.Generator().manual_seed(37)
+    for B, N, V in ((1, 3, 4090), (1, 3, 4093), (300, 8, 8189), (70, 32, 4095)):
+        wide = (torch.randn(B, N, V + 9, generator=g) * 2)
+        s = -torch.rand(B, N, generator=g) * 4
+        for dt, step in ((torch.float32, 4), (torch.bfloat16, 8)):
+            w = wide.to(dt).cuda()
+            for at in range(0, step, 1 if B == 1 else 3):
+                view = w[:, :, at:at + V]
+                a, b = decode.beam_select(view, s.cuda(), N), decode.beam_select(view.contiguous(), s.cuda(), N)
+                assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2]) and bool(((a[0] - b[0]).abs() <= 2 * 160 * U + U * b[0].abs()).all())
+            if B == 1:
+                _check_select(w[:, :, 1:1 + V].cpu().contiguous(), s, N)
 
 
 def test_select_first_step_and_dead_beams():
