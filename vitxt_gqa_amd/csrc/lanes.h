@@ -103,10 +103,9 @@ __device__ __forceinline__ double wave_sum64(double x) {
   }
   return x;
 }
-// A number that at least K of the wave's 64 lanes reach (K <= 32): the least of the maxima of G lane groups, G >= K a power of two.  Six exchanges;
-// the K-th largest itself takes a search.
-__device__ __forceinline__ uint32_t wave_kth_bound(uint32_t x, int K) {
-  const int most = K <= 1 ? 6 : 6 - (32 - __builtin_clz(K - 1));      // exchanges that take the larger: groups of 2^most lanes
+// The least of the maxima of the wave's groups of 2^most lanes: a number that 64 >> most lanes reach at least.  Six exchanges; the K-th largest
+// itself takes a search.
+__device__ __forceinline__ uint32_t wave_group_bound(uint32_t x, int most) {
   auto pick = [&](int step, uint32_t a, uint32_t b) { return step < most ? max(a, b) : min(a, b); };
   x = pick(0, x, as_u(dpp<DPP_XOR1>(as_f(x))));
   x = pick(1, x, as_u(dpp<DPP_XOR2>(as_f(x))));
