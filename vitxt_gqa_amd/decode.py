@@ -51,30 +51,61 @@ def _launch(index, fn, *args):
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _head_rows(t, name):
-    """Strides of [..., heads, 64] with dense 64-element rows that start at multiples of 4 elements (0 for axes of length 1), and its address."""
-    s = t.stride()
-    d = _DTYPES.get(t.dtype)
-    at = t.data_ptr()
-    if d is None or s[-1] != 1 or t.shape[-1] != HEAD_DIM or at & d[1] or (s[0] | s[1] | s[2] | (s[3] if len(s) == 5 else 0)) & 3:
-        _need(d is not None, "%s: float32 or bfloat16, got %s", name, t.dtype)
-        _need(t.shape[-1] == HEAD_DIM, "%s: the kernels are built for head_dim 64, got %s", name, tuple(t.shape))
-        s = tuple(x if n > 1 else 0 for x, n in zip(s[:-1], t.shape[:-1])) + (s[-1],)
-        _need(s[-1] == 1 and not at & d[1] and not any(x & 3 for x in s[:-1]),
-              "%s: rows of 64 dense elements, aligned to 4 elements, are needed (strides %s): call .contiguous()", name, t.stride())
-    return s, at
+# What follows from shapes, strides and types alone is checked and worked out once for each (calls of a few microseconds would spend as much on it).
+def _head_strides(shape, stride, dtype, name):
+    """Strides of [..., heads, 64] with dense 64-element rows that start at multiples of 4 elements (0 for axes of length 1)."""
+    _need(dtype in _DTYPES, "%s: float32 or bfloat16, got %s", name, dtype)
+    _need(shape[-1] == HEAD_DIM, "%s: the kernels are built for head_dim 64, got %s", name, tuple(shape))
+    s = tuple(x if n > 1 else 0 for x, n in zip(stride[:-1], shape[:-1]))
+    _need(stride[-1] == 1 and not any(x & 3 for x in s), "%s: rows of 64 dense elements, aligned to 4 elements, are needed (strides %s): call .contiguous()", name, stride)
+    return s
+
+
+def _aligned(name, mask, *addresses):
+    for at in addresses:
+        _need(not at & mask, "%s: rows of 64 dense elements, aligned to 4 elements, are needed (address %#x): call .contiguous()", name, at)
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_plan(B, N, H, G, max_len, dtype):
-    """(shares of the token axis, bytes of workspace) of an attention over about ``max_len`` tokens."""
-    splits = X.lib().t2s_kv8_attn_splits(B, N, H, G, max_len, dtype)
-    return splits, X.lib().t2s_kv8_attn_workspace_bytes(B, N, H, G, splits)
+def _append_layout(B, H, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype):
+    """(strides of k, strides of v, type code, alignment mask) of an append of [B, R, H, 64] rows."""
+    _need(len(k_shape) == 4 and k_shape[0] == B and k_shape[2] == H and v_shape == k_shape and v_dtype == k_dtype,
+          "append: k and v [%d, R, %d, 64] of one type, got %s %s and %s %s", B, H, tuple(k_shape), k_dtype, tuple(v_shape), v_dtype)
+    return (_head_strides(k_shape, k_stride, k_dtype, "append: k"), _head_strides(v_shape, v_stride, v_dtype, "append: v"), *_DTYPES[k_dtype])
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_layout(B, H, tokens, q_shape, q_stride, q_dtype, k_shape, k_stride, k_dtype, v_shape, v_stride, v_dtype):
+    """Of an attention over about ``tokens`` cached tokens: the strides of q and of the tails, type code, alignment mask, shapes and strides of the
+    results, shares of the token axis, bytes of workspace."""
+    _need(len(q_shape) == 4 and q_shape[0] == B and q_shape[2] > 0 and q_shape[2] % H == 0, "attend: q [%d, N, a multiple of %d, 64], got %s", B, H, tuple(q_shape))
+    sq, st, N, HQ = _head_strides(q_shape, q_stride, q_dtype, "attend: q"), (0, 0, 0, 0), q_shape[1], q_shape[2]
+    if k_shape is not None:
+        _need(len(k_shape) == 5 and k_shape == (B, N, k_shape[2], H, HEAD_DIM) and v_shape == k_shape and k_dtype == q_dtype and v_dtype == q_dtype,
+              "attend: tails [%d, %d, T, %d, 64] of q's type, got %s %s and %s %s", B, N, H, tuple(k_shape), k_dtype, tuple(v_shape), v_dtype)
+        st = _head_strides(k_shape, k_stride, k_dtype, "attend: tail_k")
+        _need(_head_strides(v_shape, v_stride, v_dtype, "attend: tail_v") == st, "attend: tail_k and tail_v need the same strides, got %s and %s", k_stride, v_stride)
+    code, mask = _DTYPES[q_dtype]
+    splits, nbytes = 1, 0
+    if N:
+        splits = X.lib().t2s_kv8_attn_splits(B, N, H, HQ // H, tokens, code)
+        nbytes = X.lib().t2s_kv8_attn_workspace_bytes(B, N, H, HQ // H, splits)
+    n = HQ * HEAD_DIM
+    return sq, st, code, mask, tuple(q_shape), (N * n, n, HEAD_DIM, 1), (B, N, HQ), (N * HQ, HQ, 1), splits, nbytes
 
 
 @functools.lru_cache(maxsize=256)
-def _select_bytes(B, N, V, K):
-    return X.lib().t2s_beam_select_workspace_bytes(B, N, V, K)
+def _select_layout(shape, stride, dtype, scores_shape, scores_dtype, finished_shape, finished_dtype, K, pad):
+    """(type code, bytes of workspace) of a selection."""
+    _need(len(shape) == 3 and shape[2] > 0 and shape[1] > 0, "beam_select: logits [B, N, V], got %s", tuple(shape))
+    B, N, V = shape
+    _need(dtype in _DTYPES, "beam_select: float32 or bfloat16 logits, got %s", dtype)
+    _need(V == 1 or stride[2] == 1, "beam_select: dense rows of logits are needed (strides %s): call .contiguous()", stride)
+    _need(scores_shape == (B, N) and scores_dtype == torch.float32, "beam_select: scores is float32 [%d, %d], got %s %s", B, N, tuple(scores_shape), scores_dtype)
+    _need(N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V, "beam_select: %d of %d x %d candidates (at most %d beams and %d candidates)", K, N, V, BEAM_MAX, BEAM_MAX)
+    _need(0 <= pad < V, "beam_select: pad %d outside the vocabulary of %d", pad, V)
+    _need(finished_shape is None or (finished_shape == (B, N) and finished_dtype in (torch.bool, torch.uint8)), "beam_select: finished is bool [%d, %d], got %s %s", B, N, finished_shape, finished_dtype)
+    return _DTYPES[dtype][0], X.lib().t2s_beam_select_workspace_bytes(B, N, V, K)
 
 
 class KVCache8:
@@ -143,8 +174,7 @@ class KVCache8:
         A value that is not finite, or a row number outside 0 .. R - 1, turns its block of that head to NaN.  Tokens that do not fit turn the
         sequence's length to -1 and every result over it to NaN, until ``set_lens`` (the lengths live on the device: nothing is waited for)."""
         B, H = self.batch, self.heads
-        if k.dim() != 4 or k.shape[0] != B or k.shape[2] != H or v.shape != k.shape or v.dtype != k.dtype:
-            _need(False, "append: k and v [%d, R, %d, 64] of one type, got %s %s and %s %s", B, H, tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
+        sk, sv, code, mask = _append_layout(B, H, k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype)
         R = T = k.shape[1]
         rp, rs, cp = None, 0, None
         if rows is not None:
@@ -157,12 +187,14 @@ class KVCache8:
         elif T > self.capacity:
             _need(False, "append: %d tokens do not fit a capacity of %d", T, self.capacity)
         _need(R > 0 or T == 0, "append: %d tokens of no rows", T)
-        (sk, kp), (sv, vp) = (_head_rows(k, "append: k"), _head_rows(v, "append: v")) if T else ((None, None),) * 2
         _same_device(self._index, k, v, counts, rows)
         if T == 0:
             return self
+        kp, vp = k.data_ptr(), v.data_ptr()
+        if (kp | vp) & mask:
+            _aligned("append", mask, kp, vp)
         X.check(_launch(self._index, X.lib().t2s_kv8_append, kp, sk[0], sk[1], sk[2], vp, sv[0], sv[1], sv[2], rp, rs, cp, *self._ptrs,
-                        self._ticket_ptr, B, H, T, R, self.blocks, _DTYPES[k.dtype][0], self._fmt), "t2s_kv8_append")
+                        self._ticket_ptr, B, H, T, R, self.blocks, code, self._fmt), "t2s_kv8_append")
         self.max_len = min(self.capacity, self.max_len + T)
         return self
 
@@ -204,37 +236,33 @@ def attend(q, cache, tail_k=None, tail_v=None, tail_len=None, scale=0.125):
 
     Codes enter the matrix pipe exactly; a query in float32 as the three bf16 terms that make it up; probabilities in 11 bits for a bfloat16
     result (which is rounded to 8), as three bf16 terms for a float32 one.  All sums, maxima and scales are float32; the result is rounded once."""
-    H = cache.heads
-    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[2] < 1 or q.shape[2] % H:
-        _need(False, "attend: q [%d, N, a multiple of %d, 64], got %s", cache.batch, H, tuple(q.shape))
-    B, N, HQ, _ = q.shape
-    sq, qp = _head_rows(q, "attend: q")
-    T, tk, tv, st, tl, tls = 0, None, None, (0, 0, 0, 0), None, (0, 0)
+    B, H, tokens = cache.batch, cache.heads, (cache.max_len + BLOCK - 1) // BLOCK * BLOCK
+    T, tk, tv, tl, tls, layout = 0, None, None, None, (0, 0), None
     if tail_k is not None and tail_v is not None:
-        T = tail_k.shape[2] if tail_k.dim() == 5 else -1
-        if tail_k.shape != (B, N, T, H, HEAD_DIM) or tail_v.shape != tail_k.shape or tail_k.dtype != q.dtype or tail_v.dtype != q.dtype:
-            _need(False, "attend: tails [%d, %d, T, %d, 64] of q's type, got %s %s and %s %s", B, N, H, tuple(tail_k.shape), tail_k.dtype, tuple(tail_v.shape), tail_v.dtype)
+        layout = _attend_layout(B, H, tokens, q.shape, q.stride(), q.dtype, tail_k.shape, tail_k.stride(), tail_k.dtype, tail_v.shape, tail_v.stride(), tail_v.dtype)
+        T = tail_k.shape[2]
         if torch.is_tensor(tail_len):
-            _need(tail_len.shape == (B, N) and tail_len.dtype == torch.int32, "attend: tail_len is an int or int32 [%d, %d]", B, N)
+            _need(tail_len.shape == layout[6][:2] and tail_len.dtype == torch.int32, "attend: tail_len is an int or int32 %s", layout[6][:2])
             tl, tls = tail_len.data_ptr(), tail_len.stride()
         elif tail_len is not None:
             T = max(0, min(int(tail_len), T))
         if T > 0:
-            st, tk = _head_rows(tail_k, "attend: tail_k")
-            sv, tv = _head_rows(tail_v, "attend: tail_v")
-            if sv != st:
-                _need(all(a == b or n == 1 for a, b, n in zip(sv, st, tail_k.shape)), "attend: tail_k and tail_v need the same strides, got %s and %s", tail_k.stride(), tail_v.stride())
+            tk, tv = tail_k.data_ptr(), tail_v.data_ptr()
     else:
         _need(tail_k is None and tail_v is None, "attend: tail_k and tail_v come together")
         _need(tail_len is None, "attend: tail_len without a tail")
+        layout = _attend_layout(B, H, tokens, q.shape, q.stride(), q.dtype, None, None, None, None, None, None)
+    sq, st, code, mask, shape, stride, lse_shape, lse_stride, splits, nbytes = layout
+    qp = q.data_ptr()
+    if (qp | (tk or 0) | (tv or 0)) & mask:
+        _aligned("attend", mask, qp, tk or 0, tv or 0)
     _same_device(cache._index, q, tail_k, tail_v, None if tl is None else tail_len)
-    dev, n = q.device, HQ * HEAD_DIM
-    out = _empty((B, N, HQ, HEAD_DIM), (N * n, n, HEAD_DIM, 1), dtype=q.dtype, device=dev)
-    lse = _empty((B, N, HQ), (N * HQ, HQ, 1), dtype=torch.float32, device=dev)
+    dev = q.device
+    out = _empty(shape, stride, dtype=q.dtype, device=dev)
+    lse = _empty(lse_shape, lse_stride, dtype=torch.float32, device=dev)
+    N, HQ = shape[1], shape[2]
     if N == 0:
         return out, lse
-    code = _DTYPES[q.dtype][0]
-    splits, nbytes = _attn_plan(B, N, H, HQ // H, cache.max_len, code)
     ws = _empty((nbytes // 4,), (1,), dtype=torch.float32, device=dev) if nbytes else None
     X.check(_launch(cache._index, X.lib().t2s_kv8_attn, qp, sq[0], sq[1], sq[2], *cache._ptrs, tk, tv, st[0], st[1], st[2], st[3], tl, tls[0], tls[1], T,
                     out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, splits, B, N, H, HQ // H, cache.blocks, scale, code, cache._fmt), "t2s_kv8_attn")
@@ -249,24 +277,14 @@ def beam_select(logits, scores, n_select, finished=None, pad=0):
     ``finished`` bool [B, N]: a beam that has ended offers the token ``pad`` at its own score and nothing else.  NaN logits count as -inf, +inf as
     the largest number.  Returns (scores [B, n_select] float32, parents int64: the beam n, tokens int64: the word v), best first, ties to the lowest
     n V + v; candidates at -inf only where nothing else is left.  At most 32 beams and 32 candidates."""
-    if logits.dim() != 3 or logits.shape[2] < 1 or logits.shape[1] < 1:
-        _need(False, "beam_select: logits [B, N, V], got %s", tuple(logits.shape))
-    B, N, V = logits.shape
-    K = int(n_select)
-    d = _DTYPES.get(logits.dtype)
-    if d is None or scores.shape != (B, N) or scores.dtype != torch.float32 or (V > 1 and logits.stride(2) != 1):
-        _need(d is not None, "beam_select: float32 or bfloat16 logits, got %s", logits.dtype)
-        _need(V == 1 or logits.stride(2) == 1, "beam_select: dense rows of logits are needed (strides %s): call .contiguous()", logits.stride())
-        _need(False, "beam_select: scores is float32 [%d, %d], got %s %s", B, N, tuple(scores.shape), scores.dtype)
-    if not (N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V and 0 <= pad < V):
-        _need(N <= BEAM_MAX and 0 < K <= BEAM_MAX and K <= N * V, "beam_select: %d of %d x %d candidates (at most %d beams and %d candidates)", K, N, V, BEAM_MAX, BEAM_MAX)
-        _need(False, "beam_select: pad %d outside the vocabulary of %d", pad, V)
-    fp = None
-    if finished is not None:
-        if finished.shape != (B, N) or (finished.dtype != torch.bool and finished.dtype != torch.uint8):
-            _need(False, "beam_select: finished is bool [%d, %d], got %s %s", B, N, tuple(finished.shape), finished.dtype)
+    K, pad, fp = int(n_select), int(pad), None
+    if finished is None:
+        code, nbytes = _select_layout(logits.shape, logits.stride(), logits.dtype, scores.shape, scores.dtype, None, None, K, pad)
+    else:
+        code, nbytes = _select_layout(logits.shape, logits.stride(), logits.dtype, scores.shape, scores.dtype, finished.shape, finished.dtype, K, pad)
         finished = finished.contiguous()
         fp = finished.data_ptr()
+    B, N, V = logits.shape
     index = logits.get_device()
     _same_device(index, logits, scores, finished)
     dev = logits.device
@@ -275,11 +293,10 @@ def beam_select(logits, scores, n_select, finished=None, pad=0):
     if B == 0:
         return out, parents, tokens
     scores = scores.contiguous()
-    nbytes = _select_bytes(B, N, V, K)
     ws = _empty(((nbytes + 7) // 8,), (1,), dtype=torch.int64, device=dev)
     sb, sn = logits.stride()[:2]
     X.check(_launch(index, X.lib().t2s_beam_select, logits.data_ptr(), sb, sn, scores.data_ptr(), fp, pad, out.data_ptr(), parents.data_ptr(),
-                    tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, d[0]), "t2s_beam_select")
+                    tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, code), "t2s_beam_select")
     return out, parents, tokens
 
 
