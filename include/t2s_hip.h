@@ -369,7 +369,7 @@ int t2s_gemm_wgrad(const void* dy, const void* x, float* dw, float* slabs, int64
  *   value of token t  byte  (t / 64) * 4096 + dim * 64 + p with t % 64 = ((p >> 2) & 3) * 16 + (p >> 4) * 4 + (p & 3)
  * amax = largest magnitude of the block (at least 2^-100); T2S_KV_INT8: s = amax / 127; T2S_KV_E4M3: s = the least power of two with
  * amax <= 448 s.  An element is held as the int8 / e4m3 number nearest to x r (r = 1 / s in fp32, exact product, ties to even) and stands for
- * code * s.  A value that is not finite makes the scale of its block NaN.  A length outside 0 .. 64 nblk (an append that did not fit
+ * code * s; a scale is positive, or NaN: a value that is not finite makes that of its block NaN.  A length outside 0 .. 64 nblk (an append that did not fit
  * leaves -1) makes every result over its sequence NaN.
  *
  * t2s_kv8_append: token j of sequence b is row rows[b, j] (NULL: row j) of k / v, element (b, row, h, d) at batch_stride b + row_stride row +
@@ -403,7 +403,7 @@ int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, in
  * t2s_beam_select: of the N V candidates scores[b, n] + logits[b, n, v] - log sum exp(logits[b, n, :]) of each sequence the n_select
  *   best, in descending order, ties to the lowest n V + v: out_scores [B, n_select] fp32, out_parents (n) and out_tokens (v) int64.
  *   logits: element (b, n, v) at batch_stride b + beam_stride n + v, fp32 or bf16; NaN counts as -inf, +inf as the largest number.
- *   finished [B, N] bytes or NULL: a beam that has ended offers `pad` at its own score and nothing else (its logits are not read).
+ *   finished [B, N] bytes or NULL: a beam that has ended offers `pad` at its own score and nothing else (its logits do not count).
  *   Candidates at -inf are taken, lowest first, only when there are no others.  Scores are formed and compared in 64 bits.
  *   N and n_select at most T2S_BEAM_MAX.  workspace: 8-byte aligned, t2s_beam_select_workspace_bytes, contents on entry irrelevant.
  * t2s_beam_reorder: state is [outer, B, N] rows of row_bytes; the first used_bytes of row (o, b, n) become those of (o, b, parents[b, n]), in place.

@@ -112,6 +112,9 @@ __device__ __forceinline__ int v_word(int tg) { return (tg & 3) * 4 + (tg >> 2);
 // append.  One workgroup = one (sequence, head) walking the blocks that the new tokens touch; a thread owns 4 tokens x 4 dims of a block, of
 // keys and of values, so both storage orders are 32-bit words of it, and the words go out through LDS images as contiguous blocks.  HBM
 // bound: the rows of the next block are on their way (their numbers, where a list names them, one block further) while a block is encoded.
+// 64 x 12 pairs, 7 000 of 10 120 listed bf16 rows of a fused projection: 458 us for 1.39 GB read and 0.70 GB written, 4.5 TB/s (keys and values in
+// workgroups of their own, nothing ahead: 619).  One token behind 84 for 48 x 12 pairs: 9.6 us, of which a workgroup's own chain - the length, the
+// rows, what the block holds, a barrier, the codes, a barrier, the store - is 5.
 struct AppendArgs {
   const void* x[2];                                // K, V
   int64_t x_bs[2], x_ts[2], x_hs[2];
@@ -437,6 +440,9 @@ __device__ __forceinline__ void tail_row(const AttnArgs& a, int b, int n, int hq
 __device__ __forceinline__ bool no_length(const AttnArgs& a, int len) { return len < 0 || len > a.nblk * KV_BLOCK; }
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * KV_LN2; }
 
+// HBM bound from a few sequences on: 64 x 12 pairs, 5 rows, 1 to 10 120 tokens: 97 to 102 us for 505 MB of codes, 5.0 TB/s, though only a third of
+// the matrix pipe's 16-row tile is in use; 2 x 8 pairs of 131 017 tokens, 4 rows: 55 to 58 us for 269 MB, 4.8 TB/s.  One sequence of 20 tokens:
+// 5.4 us, a chain of latencies.
 // One workgroup: one (sequence, head), one group of 16 QT query rows, one share of the blocks; its four waves take the blocks in turn,
 // each with its own running maximum / sum / O, and are joined through LDS at the end.  With more than one share the results go to the
 // workspace (the rows' tails are one share more, with workgroups of their own); a single share takes the tails of a few rows in as well and
@@ -675,7 +681,9 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(AttnArgs a) {
   }
 }
 
-// Joins the shares of an output row: WPR waves to a row, each with every WPR-th share; lane s weighs share s, then lane d sums dim d.
+// Joins the shares of an output row: WPR waves to a row, each with every WPR-th share; lane s weighs share s, then lane d sums dim d.  A chain of
+// two loads.  Four waves to a row where there are many shares, us with four and with one: 4 rows of 256 shares 7.2 and 19.9, 60 of 20 3.7 and 4.6,
+// 12 288 of 4 20.5 and 7.2.
 template <typename TQ, int WPR>
 __global__ __launch_bounds__(256) void kv8_attn_join_kernel(AttnArgs a) {
   __shared__ float o_s[4][KV_HD], m_s[4], l_s[4];
@@ -777,7 +785,9 @@ bool kv8_attn_shape(int B, int N, int H, int G) {
 }
 
 // Row groups of a (sequence, head), each of which reads its cache: as few as registers allow (64 rows; fp32, with three terms to everything,
-// 32), of equal size; returns the 16-row tiles of a group.
+// 32), of equal size; returns the 16-row tiles of a group.  Measured, us: 16 x 12 pairs of 4 000 tokens, bf16, 64 rows in groups of 64 30.5, 32 32.4, 16
+// 42.8; fp32, 32 rows in groups of 32 30.9, 16 33.5.  (A few pairs of 1 000 tokens, which the second-level caches hold, would be quicker in groups of 16:
+// 10.2 and 5.7.)
 int attn_row_tiles(int rows, int dtype, int* groups) {
   const int most = dtype == T2S_BF16 ? 64 : 32;
   *groups = (rows + most - 1) / most;

@@ -133,7 +133,8 @@ class KVCache8:
 
     @classmethod
     def from_parts(cls, k, v, k_scale, v_scale, lens, max_len=None):
-        """A cache around existing storage (used as it is, not copied): codes int8 or float8_e4m3fn [B, H, blocks, 64, 64], scales, lens.
+        """A cache around existing storage (used as it is, not copied): codes int8 or float8_e4m3fn [B, H, blocks, 64, 64], scales
+        (positive, or NaN for a block that holds a value that is none), lens.
         ``max_len``: a bound on the lengths, if known; it only shapes the attention's launch."""
         self = cls.__new__(cls)
         self._adopt(k, v, k_scale, v_scale, lens, max_len)
@@ -200,8 +201,8 @@ class KVCache8:
 
     def set_lens(self, lens, max_len=None):
         """Sets how many tokens each sequence holds: an int for all, or int32 [B] on the device.  Takes tokens back (a prefix is kept for another
-        continuation; 0 empties the cache); it cannot bring any in, and never more may be named than have been appended.  ``max_len`` as in
-        ``from_parts``."""
+        continuation; 0 empties the cache); it cannot bring any in, and never more may be named than have been appended.  A block that is kept in part keeps
+        its scale.  ``max_len`` as in ``from_parts``."""
         if isinstance(lens, int):
             _need(0 <= lens <= self.capacity, "set_lens: %d outside 0 .. %d", lens, self.capacity)
             self.lens.fill_(lens)

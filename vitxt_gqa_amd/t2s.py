@@ -509,10 +509,11 @@ class T2S(BaseModel):
 
     def set_decoding(self, beams=1, cache=None):
         """How eval decodes.  ``beams`` = 1, ``cache`` = None: the reference's greedy loop (t2s.py:315-354) with the prefix's K / V in the operand type.
-        ``cache`` = "int8" or "e4m3": the prefix in 8 bits (decode.KVCache8: half the memory and traffic of bf16), one new row per step.
-        ``beams`` > 1: beam search over the summed log-softmax of ``pos_scores`` (8-bit cache; "int8" unless said otherwise), a beam ending at
-        the answer processor's ``EOS_IDX`` if it has one; the output dict then also holds ``beam_tokens`` [B, beams, D] and ``beam_scores``
-        [B, beams], best first, and the three passes' scores are those along the best beam."""
+        ``cache`` = "int8" or "e4m3": the prefix in 8 bits (decode.KVCache8: half the memory and traffic of bf16), one new row per step, and beam search
+        over the summed log-softmax of ``pos_scores``; ``beams`` > 1 without a ``cache``: "int8".  A beam ends at the answer processor's ``EOS_IDX``
+        if it has one (from there on it repeats that word; the greedy loop goes on); one beam takes the greedy loop's words up to there.  The output
+        dict then also holds ``beam_tokens`` [B, beams, D] and ``beam_scores`` [B, beams], best first, and the three passes' scores are those along the
+        best beam."""
         if not 1 <= int(beams) <= 16:
             raise ValueError("set_decoding: 1 to 16 beams, got %s" % (beams,))           # (the pointer kernel takes 16 rows a sample)
         if cache is None and beams > 1:
@@ -679,7 +680,7 @@ class T2S(BaseModel):
     def _beam_decode(self, s, fwd, dt):
         """Beam search over the "pos" pass, whose scores drive the reference's loop (t2s.py:315-354), on an 8-bit cache of its prefix: a step computes
         the newest row of every beam, picks the best continuations of all beams and moves the beams' states to where they come from.  The
-        three passes' scores are then computed along the best beam, all decoder rows at once.  One beam: the greedy loop."""
+        three passes' scores are then computed along the best beam, all decoder rows at once.  One beam: the greedy loop up to the answer's end."""
         g = self.Grounding_Module
         txt, obj, ocr = fwd["txt_emb"], fwd["obj_mmt_in"], fwd["ocr_mmt_in"]
         B, T, Fn, L1 = txt.size(0), txt.size(1), obj.size(1), txt.size(1) + obj.size(1) + ocr.size(1)
