@@ -31,7 +31,7 @@ constexpr int BS_MAX = T2S_BEAM_MAX;               // beams, and candidates to s
 constexpr int BS_EPT = 16;                         // elements of a thread per stretch
 constexpr int BS_SUB = 256 * BS_EPT;
 constexpr int BS_CHUNKS = 32;                      // workgroups of a row at most
-constexpr int BS_WGS = 2048;                       // workgroups about (384 rows of 30 522 bf16 logits: 1 152 17.6 us, 1 536 16.4, 3 072 22.0)
+constexpr int BS_WGS = 2048;                       // workgroups about (384 rows of 30 522 bf16 logits: 3 to a row 17.6 us, 4 16.4, 8 22.0)
 constexpr int BS_LIST = 256;                       // logits of a wave that are ranked without more ado
 
 // order-preserving unsigned form of a float (-inf < ... < -0 = +0 < ... < max)
