@@ -715,6 +715,80 @@ def test_captured_step_replays():
         assert torch.equal(a, b)
 
 
+def test_threads_on_streams_of_their_own():
+    """Two threads, each with a stream, a cache and beams of its own, at the same time: what each gets alone."""
+    import threading
+    from vitxt_gqa_amd import decode
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        L, N = 900 + 700 * seed, 2 + seed
+        return [t.cuda() for t in (_rows(g, 3, L, 2, HD), _rows(g, 3, L, 2, HD), _rows(g, 3, N, 4, HD), torch.randn(3, N, 9000 + seed, generator=g), -torch.rand(3, N, generator=g), torch.randn(3, N, 500, generator=g))]
+
+    def work(x, rounds):
+        out = []
+        for _ in range(rounds):
+            cache = decode.KVCache8(3, 2, x[0].shape[1], "int8")
+            cache.append(x[0][:, :333], x[1][:, :333]).append(x[0][:, 333:], x[1][:, 333:])
+            state = x[5].clone()
+            s, p, t = decode.beam_select(x[3], x[4], x[4].shape[1])
+            out.append((*decode.attend(x[2], cache), s, p, t, decode.beam_reorder(state, p), cache.lens.clone()))
+        return out
+
+    data = [inputs(0), inputs(1)]
+    want = [work(x, 1)[0] for x in data]
+    torch.cuda.synchronize()
+    got, go = [None, None], threading.Barrier(2)
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            go.wait()
+            got[i] = work(data[i], 25)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert got[i] is not None and len(got[i]) == 25
+        for res in got[i]:
+            for a, b in zip(res, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_two_graphs_of_one_pool():
+    """Two captured graphs whose workspaces come from one pool, replayed in turn with eager calls between: each replay gives what its inputs give."""
+    from vitxt_gqa_amd import decode
+    g = torch.Generator().manual_seed(43)
+    caches = [_filled(g, 2, 2, [3000, 1234]), _filled(g, 1, 1, [20000], "e4m3")]
+    shapes = [((2, 5, 4, HD), (2, 5, 7001)), ((1, 2, 1, HD), (1, 2, 70000))]
+    bufs = [(torch.zeros(a).cuda(), torch.zeros(b).cuda(), torch.zeros(b[:2]).cuda()) for a, b in shapes]
+    call = lambda i, x: (*decode.attend(x[0], caches[i]), *decode.beam_select(x[1], x[2], 3))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i in range(2):
+            call(i, bufs[i])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    with torch.cuda.graph(graphs[0]):
+        outs.append(call(0, bufs[0]))
+    with torch.cuda.graph(graphs[1], pool=graphs[0].pool()):
+        outs.append(call(1, bufs[1]))
+    for turn in range(6):
+        for i in ((0, 1), (1, 0), (0, 0), (1, 1), (1, 0), (0, 1))[turn]:
+            x = [torch.randn(b.shape, generator=g).cuda() for b in bufs[i]]
+            want = call(i, x)
+            for b, t in zip(bufs[i], x):
+                b.copy_(t)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs[i], want):
+                assert torch.equal(a, b), (turn, i)
+
+
 def test_gradients_are_refused():
     from vitxt_gqa_amd import decode
     cache = decode.KVCache8(1, 1, 64)
