@@ -138,15 +138,15 @@ def test_c_abi_refuses(lib):
         a = list(att)
         a[i] = v
         assert lib.t2s_kv8_attn(*a) != 0 and text in lib.t2s_last_error(), (i, lib.t2s_last_error())
-    sel = [p, 5, 5, p, None, 0, p, p, p, p, 1 << 20, 1, 3, 5, 3, 0, None]
-    for i, v, text in ((0, None, b"null pointer"), (12, 33, b"bad shape"), (14, 16, b"candidates"), (5, 5, b"pad"), (10, 8, b"too small"), (15, 2, b"bad dtype")):
+    sel = [p, 40000, 40000, p, None, 0, p, p, p, p, 1 << 20, 1, 3, 40000, 3, 0, None]
+    for i, v, text in ((0, None, b"null pointer"), (12, 33, b"bad shape"), (14, 33, b"candidates"), (5, 40000, b"pad"), (10, 8, b"too small"), (15, 2, b"bad dtype")):
         a = list(sel)
         a[i] = v
         assert lib.t2s_beam_select(*a) != 0 and text in lib.t2s_last_error(), (i, lib.t2s_last_error())
     assert lib.t2s_beam_reorder(p, p, 1, 1, 33, 16, 16, None) != 0 and b"bad shape" in lib.t2s_last_error()
     assert lib.t2s_beam_reorder(p, p, 1, 1, 3, 16, 32, None) != 0 and b"bytes" in lib.t2s_last_error()
     assert lib.t2s_kv8_attn_splits(0, 1, 1, 1, 64, 0) == 0 and lib.t2s_kv8_attn_splits(1, 1, 1, 1, 0, 1) == 1
-    assert lib.t2s_beam_select_workspace_bytes(0, 1, 1, 1) == 0
+    assert lib.t2s_beam_select_workspace_bytes(0, 1, 1, 1) == 0 == lib.t2s_beam_select_workspace_bytes(1, 5, 5600, 5) < lib.t2s_beam_select_workspace_bytes(1, 3, 40000, 3)
     # shapes whose products pass 32 bits are refused, none ends the process
     big = 2 ** 31 - 1
     assert lib.t2s_kv8_attn_splits(1, 65536, 1, 65536, 64, 0) == 0 and lib.t2s_kv8_attn_splits(big, 1, big, 1, 64, 0) == 0 and lib.t2s_kv8_attn_splits(1, 1, 1, 1, big, 0) > 1
@@ -156,7 +156,7 @@ def test_c_abi_refuses(lib):
         a[25], a[26], a[27] = n, h, grp
         assert lib.t2s_kv8_attn(*a) != 0 and b"bad shape" in lib.t2s_last_error()
     a = list(sel)
-    a[10:13] = big, 1 << 24, 3
+    a[10:14] = big, 1 << 24, 3, 40000
     assert lib.t2s_beam_select(*a) != 0 and (b"too many rows" in lib.t2s_last_error() or b"too small" in lib.t2s_last_error())
     assert lib.t2s_beam_reorder(p, p, 1, 1, 3, 1 << 40, 1 << 40, None) != 0 and b"too long" in lib.t2s_last_error()
 

@@ -504,24 +504,59 @@ def test_select_in_orders_that_defeat_the_bound(order):
             _check_select_ordered(x.to(dt), torch.zeros(2, N), K)
 
 
-def _check_select_ordered(x, s, K):
+def _check_select_ordered(x, s, K, finished=None, pad=0):
     """The statement's order wherever its scores differ clearly; equal logits of a row in the order of their places."""
     from vitxt_gqa_amd import decode
-    got, p, t = (r.cpu() for r in decode.beam_select(x.cuda(), s.cuda(), K))
-    best, rp, rt = select_ref(x, s, K)
+    got, p, t = (r.cpu() for r in decode.beam_select(x.cuda(), s.cuda(), K, None if finished is None else finished.cuda(), pad))
+    best, rp, rt = select_ref(x, s, K, finished, pad)
     ref = best[:, :K]
     inf = ref == -math.inf
     assert torch.equal(got.double() == -math.inf, inf) and bool(((got.double() - ref).abs() <= 160 * U + U * ref.abs())[~inf].all())
-    total = (s.double()[..., None] + torch.log_softmax(x.double(), -1)).flatten(1)
-    V = x.shape[2]
+    V, N = x.shape[2], x.shape[1]
+    full = select_ref(x, s, N * V, finished, pad)                                  # every candidate's score, at its place
+    total = torch.empty_like(full[0]).scatter_(1, full[1] * V + full[2], full[0])
     for b in range(x.shape[0]):
         picked = (p[b] * V + t[b]).tolist()
-        assert len(set(picked)) == K and all(0 <= w < V for w in t[b].tolist())
+        assert len(set(picked)) == K and all(0 <= w < V for w in t[b].tolist()) and all(0 <= n < N for n in p[b].tolist())
         mine = total[b, picked]
+        assert torch.equal(mine == -math.inf, inf[b])
         assert bool(((mine - ref[b])[~inf[b]].abs() <= 2 * 160 * U).all())         # a permutation among scores that are equal up to the tolerance at most
         for i in range(1, K):
-            if p[b, i] == p[b, i - 1] and x[b, p[b, i], t[b, i]] == x[b, p[b, i], t[b, i - 1]]:
+            # (beside an infinite logit, which counts as 3.4e38, every x - 3.4e38 is -3.4e38 in 64 bits: not a tie of the logits)
+            if p[b, i] == p[b, i - 1] and mine[i] == mine[i - 1] and x[b, p[b, i]].max() < math.inf:
                 assert t[b, i] > t[b, i - 1]
+        assert picked[int((~inf[b]).sum()):] == (rp[b] * V + rt[b]).tolist()[int((~inf[b]).sum()):]      # at -inf: the lowest places
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("N,V", [(32, 1), (1, 33), (32, 1024), (31, 1024), (16, 2048), (1, 32768), (4, 8192), (5, 6144), (3, 10241), (8, 4097), (13, 63), (2, 16384), (2, 16385), (32, 1025)])
+def test_select_few_logits(dtype, N, V):
+    """Sequences on either side of what one workgroup holds: all beams alike, one beam, masked, tied, ended, in falling order, hardly a number left."""
+    g = torch.Generator().manual_seed(38 + N + V)
+    x = (torch.randn(3, N, V, generator=g) * 2).to(DT[dtype])
+    s = -torch.rand(3, N, generator=g) * 6
+    fin = torch.rand(3, N, generator=g) < 0.4
+    first = torch.full((3, N), -math.inf)
+    first[:, 0] = 0.0
+    apart = -torch.arange(N).float().expand(3, N) * 7                                           # one beam far ahead of the others
+    for K in sorted({1, min(5, N * V), min(N, N * V), min(32, N * V)}):
+        _check_select_ordered(x, s, K)
+        _check_select_ordered(x, s, K, fin, V - 1)
+        _check_select_ordered(x, first, K)
+        _check_select_ordered(x, apart, K)
+        _check_select_ordered(x, apart.flip(1), K, fin, V // 3)
+        _check_select_ordered(x, torch.zeros(3, N), K, torch.ones(3, N, dtype=torch.bool), V // 2)
+        _check_select_ordered(x.masked_fill(torch.rand(3, N, V, generator=g) < 0.97, -math.inf), s, K, fin, 0)
+        _check_select_ordered(torch.zeros_like(x), torch.zeros(3, N), K)
+        _check_select_ordered((x / 2).round(), s, K)
+        _check_select_ordered(torch.sort(x, -1, descending=True).values, s, K)
+        _check_select_ordered(x.masked_fill(torch.rand(3, N, V, generator=g) < 0.5, torch.finfo(DT[dtype]).min), s, K)
+        comb = x + 40 * (torch.arange(V) % 64 < 33).to(x.dtype)                                 # the best logits of a wave in few lanes
+        _check_select_ordered(comb, s, K)
+        _check_select_ordered((comb / 16).round(), s, K, fin, V // 2)
+        bad = x.clone()
+        bad[0, 0, V // 3], bad[1, N - 1, V - 1], bad[2, N // 2, 0] = math.nan, math.inf, math.nan
+        _check_select_ordered(bad, s, K)
 
 
 def test_select_rows_that_start_anywhere():

@@ -11,10 +11,10 @@
 // unique, so "descending, ties to the lowest index" is plain integer order, and there is no tie to handle anywhere.  A workgroup
 // holds a stretch of a row in registers, keeps its running maximum / sum of exponentials and its `select` best keys; a second kernel
 // joins the stretches of a sequence and orders the candidates of its N rows by their scores in 64 bits (rows differ by
-// cum - log-sum-exp, which 32 bits would merge into false ties).
+// cum - log-sum-exp, which 32 bits would merge into false ties).  Sequences of few logits are one workgroup's, in one launch (below).
 //
-// Latencies bound both kernels at a beam search's sizes: a stretch of 4 096 logits takes a workgroup 4 us on its own (its logits 2 500 cycles, maxima and
-// sums 600, the bound 800, listing 2 300, ranking 1 500).  Rows and join, us: one sequence of 5 beams x 5 600 fp32 logits 5.9 + 3.7, 64 x 5 x 15 000
+// Latencies bound all of it at a beam search's sizes: a stretch of 4 096 logits takes a workgroup 4 us on its own (its logits 2 500 cycles, maxima and
+// sums 600, the bound 800, listing 2 300, ranking 1 500).  Rows and join, us: 64 x 5 x 15 000
 // fp32 11.5 + 5.1 (15.4 MB), 48 x 8 x 30 522 bf16 16.4 + 7.0 (21.1 MB).  Requesting the next stretch's logits while one is worked on costs a CU one of
 // its six workgroups: 19.5 instead of 16.4.
 #include <algorithm>
@@ -267,6 +267,11 @@ __device__ __forceinline__ uint64_t ordered64(double x) {
 }
 __device__ __forceinline__ double from_ordered64(uint64_t k) { return __builtin_bit_cast(double, k >> 63 ? k ^ 1ull << 63 : ~k); }
 
+// log s of a normal s > 0, off by 2^-24 at most (the exponentials in s are off by as much), 0 for 1: the 64-bit function takes a workgroup a microsecond
+__device__ __forceinline__ double log_of(double s) {
+  return ((double)__builtin_amdgcn_frexp_exp(s) + (double)__builtin_amdgcn_logf((float)__builtin_amdgcn_frexp_mant(s))) * 0.69314718055994531;
+}
+
 // one workgroup per sequence: joins the stretches, orders the N rows' candidates, 256 BJ_PER of them at a time
 __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restrict__ keys, const double* __restrict__ sums, const float* __restrict__ maxs,
                                                         const float* __restrict__ cum, const uint8_t* __restrict__ finished, float* __restrict__ out_scores,
@@ -302,7 +307,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
     }
     const double cd = c0 > -INFINITY ? (double)fminf(c0, 3.402823466e38f) : -INFINITY;
     top_m[tid] = ended ? 0.f : m;
-    off_s[tid] = ended || !(s > 0.0) ? cd : cd - log(s);
+    off_s[tid] = ended || !(s > 0.0) ? cd : cd - log_of(s);
   }
   if (tid < K) top_s[tid] = none;
   __syncthreads();
@@ -373,6 +378,235 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
+// Few logits to a sequence: one launch, one workgroup of 16 waves per sequence, which holds all of its logits in registers.  A wave has up to 2 048
+// consecutive logits of a row, 32 to a lane, 64 apart (every lane has some also of a short row).  With the rows' sums known, the least of the best scores
+// of G >= K lane groups is a bound that K scores reach: groups of the whole workgroup where its rows are alike, of one wave where a row is far ahead,
+// whichever is larger (where groups have no number, the K-th largest itself of 64 groups' best scores, or of a wave's lanes').  Only what reaches it is
+// listed and ranked.  Where the list does not hold that (ties, hardly a logit left) there are two slower ways.
+// The code is run once, by few workgroups: a good part of the time goes into fetching it, so what need not be unrolled is not.
+constexpr int BW_WAVES = 16, BW_EPT = 32, BW_PIECE = 64 * BW_EPT, BW_LIST = 64 * BW_WAVES;
+
+// A bound that the K largest of the wave's 64 numbers reach, and no others unless they equal the K-th; 0 where fewer than K are not zero
+__device__ __forceinline__ uint32_t wave_kth32(uint32_t key, int K) {
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    const uint32_t t1 = t | 1u << bit, t2 = t | 2u << bit, t3 = t | 3u << bit;
+    const int c1 = __popcll(__ballot(key >= t1)), c2 = __popcll(__ballot(key >= t2)), c3 = __popcll(__ballot(key >= t3));
+    t = c3 >= K ? t3 : c2 >= K ? t2 : c1 >= K ? t1 : t;
+    if (c1 == K || c2 == K || c3 == K) break;
+  }
+  return t;
+}
+
+template <typename TX>
+__global__ __launch_bounds__(64 * BW_WAVES) void beam_whole_kernel(const TX* __restrict__ logits, int64_t l_bs, int64_t l_ns, const float* __restrict__ cum,
+                                                                   const uint8_t* __restrict__ finished, float* __restrict__ out_scores,
+                                                                   int64_t* __restrict__ out_parents, int64_t* __restrict__ out_tokens, int N, int V, int K,
+                                                                   int pad, int pieces) {
+  __shared__ Cand list_s[BW_LIST], best_s[BW_WAVES];
+  __shared__ double part_s[BW_WAVES];
+  __shared__ float part_m[BW_WAVES];
+  __shared__ uint32_t low_s[64], most_s;
+  __shared__ int cnt_s, rank_s[BW_LIST];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, b = blockIdx.x;
+  const bool busy = wave < N * pieces;             // (the same for the whole wave, like row, at, c, ended, dead)
+  const int row = busy ? wave / pieces : 0, at = busy ? (wave - row * pieces) * BW_PIECE : V;
+  const TX* x = logits + (int64_t)b * l_bs + (int64_t)row * l_ns;
+  float val[BW_EPT];
+#pragma unroll
+  for (int i = 0; i < BW_EPT; ++i) {
+    const int v = at + i * 64 + lane;
+    val[i] = v < V ? (float)x[v] : -INFINITY;
+  }
+  const float c = cum[(int64_t)b * N + row];
+  const bool ended = finished && finished[(int64_t)b * N + row], dead = !(c > -INFINITY);
+  rank_s[tid] = 0;
+  if (tid == 0) {
+    cnt_s = 0;
+    most_s = 0;
+  }
+  // An ended row is one of a single word, a dead one of none.  The word changes places with word 0: it is the first logit of the row's first lane.
+  if (dead || ended) {
+#pragma unroll
+    for (int i = 0; i < BW_EPT; ++i) val[i] = -INFINITY;
+    if (!dead && at + lane == 0) val[0] = 0.f;
+  }
+  auto word = [&](int i) {
+    const int v = at + i * 64 + lane;
+    return ended ? (v == 0 ? pad : v == pad ? 0 : v) : v;
+  };
+  float m = -INFINITY, mx = -INFINITY;
+  double sum = 0.0;
+  if (busy) {
+#pragma unroll 1
+    for (int pass = 0;; ++pass) {                  // (NaN and +inf are taken out where a NaN sum shows them, as above)
+      mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < BW_EPT; ++i) mx = fmaxf(mx, val[i]);
+      m = wave_max(mx);
+      const float mu = m > -INFINITY ? m : 0.f;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < BW_EPT; ++i) s += __expf(val[i] - mu);
+      sum = wave_sum64((double)s);
+      if (pass || sum == sum) break;
+#pragma unroll
+      for (int i = 0; i < BW_EPT; ++i) val[i] = clean(val[i]);
+    }
+  }
+  if (lane == 0) {
+    part_m[wave] = m;
+    part_s[wave] = sum;
+  }
+  __syncthreads();
+  // the row's maximum and sum from its waves', and what its logits' scores are relative to
+  const float m_part = lane < pieces ? part_m[row * pieces + lane] : -INFINITY, m_row = wave_max(m_part);
+  const double s_row = wave_sum64(m_part > -INFINITY ? part_s[row * pieces + lane] * (double)__expf(m_part - m_row) : 0.0);
+  const double cd = dead ? -INFINITY : (double)fminf(c, 3.402823466e38f), top = m_row, off = s_row > 0.0 ? cd - log_of(s_row) : cd;
+  auto score = [&](float x) { return x > -INFINITY ? off + ((double)x - top) : -INFINITY; };
+  const uint32_t mine = ordered((float)score(mx));
+  const int most = 6 - (K <= 1 ? 0 : 32 - __builtin_clz(K - 1));       // (64 / 2^most = G)
+  uint32_t low = wave_group_bound(mine, most), group = mine;
+  group = max(group, as_u(dpp<DPP_XOR1>(as_f(group))));
+  group = max(group, as_u(dpp<DPP_XOR2>(as_f(group))));
+  group = max(group, as_u(dpp<DPP_ROR4>(as_f(group))));
+  group = max(group, as_u(dpp<DPP_ROR8>(as_f(group))));
+  if ((lane & 15) == 0) low_s[wave * 4 + (lane >> 4)] = group;
+  if (lane == 0) atomicMax(&most_s, low);
+  __syncthreads();
+  group = low_s[lane];
+  low = max(wave_group_bound(group, most), most_s);
+  if (low <= 0x7fffffu && 4 * N * pieces >= K) low = wave_kth32(group, K);
+  if (low <= 0x7fffffu) {                          // (-inf's form; the same for all waves)
+    low = wave_kth32(mine, K);
+    if (lane == 0) atomicMax(&most_s, low);
+    __syncthreads();
+    low = most_s;
+  }
+  // (read once more: taking it from the registers is a choice among all of them)
+  auto logit = [&](int i) { return dead || ended ? (!dead && at + lane + i == 0 ? 0.f : -INFINITY) : clean((float)x[at + i * 64 + lane]); };
+  auto list = [&](uint32_t mask) {
+    int to = 0;
+    if (mask) to = atomicAdd(&cnt_s, __popc(mask));
+#pragma unroll 1
+    for (; mask; mask &= mask - 1, ++to) {
+      const int i = __builtin_ctz(mask);
+      const uint64_t sc = ordered64(score(logit(i)));
+      if (to < BW_LIST) list_s[to] = Cand{sc, ~((uint64_t)row << 32 | (uint32_t)word(i))};
+    }
+  };
+  bool listed = low > 0x7fffffu;                   // (or no wave has K numbers)
+  if (listed) {
+    // Scores of 64 bits whose fp32 rounding reaches `low` belong to logits above thr: low's half step, and the roundings of thr itself, are taken off it
+    const double f = (double)from_ordered(low), t = top + (f - off);
+    float thr = (float)(t - (fabs(f) * 0x1p-23 + (fabs(t) + fabs(off) + fabs(top)) * 0x1p-50));
+    thr = thr == 0.f ? -0.0f : fmaxf(thr, -3.402823466e38f);           // (the sign of x - thr: -0 - 0 would have one, -inf - -inf need not)
+    uint32_t below = 0;
+#pragma unroll
+    for (int i = BW_EPT - 1; i >= 0; --i) below = __builtin_amdgcn_alignbit(below, as_u(val[i] - thr), 31);
+    list(off > -INFINITY ? ~below : 0);
+    __syncthreads();
+    listed = cnt_s <= BW_LIST;
+  }
+  uint32_t left = 0;                               // the lane's logits that are there and not taken
+#pragma unroll
+  for (int i = 0; i < BW_EPT; ++i) left |= at + i * 64 + lane < V ? 1u << i : 0u;
+  // the best of them: the largest logit, of equal ones the first word (in an ended row word 0 is ahead of the lane's other masked words); -1: none left
+  auto look = [&]() {
+    float bx = -INFINITY;
+    int bi = -1;
+#pragma unroll
+    for (int i = 0; i < BW_EPT; ++i)
+      if ((left >> i & 1) && (bi < 0 || val[i] > bx)) {
+        bx = val[i];
+        bi = i;
+      }
+    const int swapped = pad - at - lane;
+    if (ended && bx == -INFINITY && swapped >= 0 && swapped < BW_PIECE && swapped % 64 == 0 && (left >> swapped / 64 & 1)) bi = swapped / 64;
+    return bi;
+  };
+  if (!listed) {
+    // Second try, with words for ties: of each wave what reaches its K-th best of one key a lane (keys are unique: K lanes do), and the best wave's K-th score
+    __syncthreads();
+    const int bi = look();
+    auto key_of = [&](int i, float x) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - (uint32_t)word(i)); };
+    const uint64_t thr = wave_kth(bi < 0 ? 0 : key_of(bi, logit(bi)), K, 0);
+    const uint32_t hi = (uint32_t)(thr >> 32);
+    if (lane == 0) best_s[wave].score = thr == 1 ? 0 : ordered64(hi > 0x7fffffu ? score(from_ordered(hi)) : -INFINITY);
+    if (tid == 0) cnt_s = 0;
+    __syncthreads();
+    uint64_t kth = 0;
+#pragma unroll
+    for (int w = 0; w < BW_WAVES; ++w) kth = max(kth, best_s[w].score);
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = 0; i < BW_EPT; ++i) mask |= (left >> i & 1) && key_of(i, val[i]) >= thr && ordered64(score(val[i])) >= kth ? 1u << i : 0u;
+    list(mask);
+    __syncthreads();
+    listed = cnt_s <= BW_LIST;
+  }
+  if (listed) {
+    // a lane to a candidate, the others to compare it with shared by as many waves as there are
+    const int cnt = cnt_s, across = (cnt + 63) >> 6, share = wave / across, shares = BW_WAVES / across, at = (wave - share * across) * 64 + lane;
+    if (share < shares && at < cnt) {
+      const Cand x = list_s[at];
+      const int each = (cnt + shares - 1) / shares, to_j = min(cnt, (share + 1) * each);
+      int rank = 0;
+#pragma unroll 4
+      for (int j = share * each; j < to_j; ++j) rank += before(list_s[j], x);
+      if (rank) atomicAdd(rank_s + at, rank);
+    }
+    __syncthreads();
+    if (tid < cnt && rank_s[tid] < K) {
+      const Cand r = list_s[tid];
+      const int64_t to = (int64_t)b * K + rank_s[tid];
+      out_scores[to] = (float)from_ordered64(r.score);
+      out_parents[to] = (int64_t)(~r.place >> 32);
+      out_tokens[to] = (int64_t)(~r.place & 0xffffffffu);
+    }
+    return;
+  }
+  // third try, where a few lanes have most of the best logits: one by one
+  Cand own{0, 0};
+  int bi = -1;
+  bool stale = true;                               // the lane's best has been taken (its wave looks again, the others' bests stand)
+#pragma unroll 1
+  for (int k = 0; k < K; ++k) {
+    if (__any(stale)) {
+      if (stale) {
+        bi = look();
+        own = bi < 0 ? Cand{0, 0} : Cand{ordered64(score(logit(bi))), ~((uint64_t)row << 32 | (uint32_t)word(bi))};
+        stale = false;
+      }
+      Cand y = own;
+#pragma unroll 1
+      for (int i = 32; i > 0; i >>= 1) {
+        const Cand z{__shfl_xor(y.score, i, 64), __shfl_xor(y.place, i, 64)};
+        if (before(z, y)) y = z;
+      }
+      if (lane == 0) best_s[wave] = y;
+    }
+    __syncthreads();
+    Cand y = best_s[0];
+#pragma unroll
+    for (int w = 1; w < BW_WAVES; ++w)
+      if (before(best_s[w], y)) y = best_s[w];
+    if (bi >= 0 && own.place == y.place) {
+      left &= ~(1u << bi);
+      stale = true;
+    }
+    if (tid == 0) {
+      const int64_t to = (int64_t)b * K + k;
+      out_scores[to] = (float)from_ordered64(y.score);
+      out_parents[to] = (int64_t)(~y.place >> 32);
+      out_tokens[to] = (int64_t)(~y.place & 0xffffffffu);
+    }
+    __syncthreads();                               // (best_s is written again)
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
 // in place: a thread owns one unit of bytes of every beam of a sequence, loads all of them from where they come and only then stores.  Bound by
 // bandwidth where there is much (64 x 5 beams of 3 x 36 KB: 8.7 us for 57 MB that the caches hold, 17.4 when the beams went through scratch memory), by
 // the chain parents - load - store otherwise (2.9 us).
@@ -420,10 +654,18 @@ void beam_chunks(int64_t rows, int64_t V, int* chunks, int* subs) {
   *chunks = (n + *subs - 1) / *subs;
 }
 
+// Waves of a row where a sequence is a workgroup's, 0 where it has too many logits for one.  Measured, us, one workgroup and rows + join (and a launch
+// less, 3 us of the host's): 1 x 5 beams of 5 600 logits 7.2 and 5.7 + 3.6, 64 of them 8.6 and 7.7 + 4.5, 1 024 35.3 and 34.9 + 4.8; 64 x 16 x 2 048 9.0 and
+// 13.8 + 5.0; 8 x 1 x 32 768, 32 best 9.5 and 13.6 + 8.0; 1 x 1 x 50 5.2 and 4.2 + 2.9.  All logits equal: 31 and 31 + 4.4.
+int beam_pieces(int64_t N, int64_t V) {
+  const int64_t pieces = (V + BW_PIECE - 1) / BW_PIECE;
+  return N * pieces <= BW_WAVES ? (int)pieces : 0;
+}
+
 }  // namespace
 
 extern "C" int64_t t2s_beam_select_workspace_bytes(int B, int N, int V, int n_select) {
-  if (B <= 0 || N <= 0 || V <= 0 || n_select <= 0) return 0;
+  if (B <= 0 || N <= 0 || V <= 0 || n_select <= 0 || beam_pieces(N, V)) return 0;
   int chunks = 0, subs;
   for (int skew : {0, 3, 7}) {                     // (more words may make fewer workgroups of more stretches)
     int c;
@@ -436,7 +678,7 @@ extern "C" int64_t t2s_beam_select_workspace_bytes(int B, int N, int V, int n_se
 extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t beam_stride, const float* scores, const uint8_t* finished,
                                int pad, float* out_scores, int64_t* out_parents, int64_t* out_tokens, void* workspace, int64_t workspace_bytes,
                                int B, int N, int V, int n_select, int dtype, t2s_stream_t stream) {
-  T2S_CHECK_ARG(logits && scores && out_scores && out_parents && out_tokens && workspace, "beam_select: null pointer");
+  T2S_CHECK_ARG(logits && scores && out_scores && out_parents && out_tokens && (workspace || !workspace_bytes), "beam_select: null pointer");
   T2S_CHECK_ARG(B > 0 && N > 0 && N <= BS_MAX && V > 0 && V <= 0x7ffffff0, "beam_select: bad shape B=%d N=%d V=%d (at most %d beams)", B, N, V, BS_MAX);
   T2S_CHECK_ARG(n_select > 0 && n_select <= BS_MAX && n_select <= (int64_t)N * V, "beam_select: %d of %d x %d candidates (at most %d)", n_select, N, V, BS_MAX);
   T2S_CHECK_ARG(pad >= 0 && pad < V, "beam_select: pad %d outside the vocabulary of %d", pad, V);
@@ -444,6 +686,18 @@ extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t
   T2S_CHECK_ARG((uintptr_t)logits % (dtype == T2S_F32 ? 4 : 2) == 0, "beam_select: logits not aligned to their type");
   T2S_CHECK_ARG((uintptr_t)workspace % 8 == 0 && workspace_bytes >= t2s_beam_select_workspace_bytes(B, N, V, n_select), "beam_select: workspace of %lld bytes is too small",
                 (long long)workspace_bytes);
+  hipStream_t st = (hipStream_t)stream;
+  if (const int pieces = beam_pieces(N, V)) {
+    T2S_CHECK_ARG(B < (1 << 22), "beam_select: too many sequences");
+    if (dtype == T2S_BF16)
+      hipLaunchKernelGGL(beam_whole_kernel<bf16_t>, dim3((unsigned)B), dim3(64 * BW_WAVES), 0, st, (const bf16_t*)logits, batch_stride, beam_stride, scores, finished, out_scores,
+                         out_parents, out_tokens, N, V, n_select, pad, pieces);
+    else
+      hipLaunchKernelGGL(beam_whole_kernel<float>, dim3((unsigned)B), dim3(64 * BW_WAVES), 0, st, (const float*)logits, batch_stride, beam_stride, scores, finished, out_scores,
+                         out_parents, out_tokens, N, V, n_select, pad, pieces);
+    T2S_CHECK_LAUNCH("beam_select");
+    return 0;
+  }
   const int64_t es = dtype == T2S_F32 ? 4 : 2;
   const bool whole = (uintptr_t)logits % 16 == 0 && batch_stride * es % 16 == 0 && beam_stride * es % 16 == 0;
   int chunks, subs;
@@ -453,7 +707,6 @@ extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t
   uint64_t* keys = (uint64_t*)workspace;
   double* sums = (double*)(keys + grid * n_select);
   float* maxs = (float*)(sums + grid);
-  hipStream_t st = (hipStream_t)stream;
   if (dtype == T2S_BF16)
     hipLaunchKernelGGL(beam_rows_kernel<bf16_t>, dim3((unsigned)grid), dim3(256), 0, st, (const bf16_t*)logits, batch_stride, beam_stride, scores, finished, keys, sums, maxs,
                        N, V, n_select, pad, chunks, subs);

@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
   swap32(as_f(max(as_u(a), as_u(b))), a, b);
   return max(as_u(a), as_u(b));
 }
-// maximum / sum over the wave's sixteen quads, each of which holds one value four times
+// maximum / sum over the wave's sixteen quads, each of which holds one value four times (the sum's last bit may differ from lane to lane)
 __device__ __forceinline__ float quads_max(float x) {
   x = fmaxf(x, dpp<DPP_ROR4>(x));
   x = fmaxf(x, dpp<DPP_ROR8>(x));
@@ -76,7 +76,7 @@ __device__ __forceinline__ float wave_max(float x) {
   x = fmaxf(x, dpp<DPP_XOR2>(x));
   return quads_max(x);
 }
-// sum over the wave, in 64 bits
+// sum over the wave, in 64 bits; the same bits in every lane (the rings add in another order in each)
 template <int CTRL>
 __device__ __forceinline__ double dpp64(double x) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x);
@@ -101,7 +101,9 @@ __device__ __forceinline__ double wave_sum64(double x) {
     }
     x = __builtin_bit_cast(double, (uint64_t)as_u(h0) << 32 | as_u(l0)) + __builtin_bit_cast(double, (uint64_t)as_u(h1) << 32 | as_u(l1));
   }
-  return x;
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32)), lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 // The least of the maxima of the wave's groups of 2^most lanes: a number that 64 >> most lanes reach at least.  Six exchanges; the K-th largest
 // itself takes a search.

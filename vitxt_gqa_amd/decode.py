@@ -294,10 +294,10 @@ def beam_select(logits, scores, n_select, finished=None, pad=0):
     if B == 0:
         return out, parents, tokens
     scores = scores.contiguous()
-    ws = _empty(((nbytes + 7) // 8,), (1,), dtype=torch.int64, device=dev)
+    ws = _empty(((nbytes + 7) // 8,), (1,), dtype=torch.int64, device=dev) if nbytes else None
     sb, sn = logits.stride()[:2]
     X.check(_launch(index, X.lib().t2s_beam_select, logits.data_ptr(), sb, sn, scores.data_ptr(), fp, pad, out.data_ptr(), parents.data_ptr(),
-                    tokens.data_ptr(), ws.data_ptr(), nbytes, B, N, V, K, code), "t2s_beam_select")
+                    tokens.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, B, N, V, K, code), "t2s_beam_select")
     return out, parents, tokens
 
 
