@@ -407,7 +407,7 @@ __global__ __launch_bounds__(64 * BW_WAVES) void beam_whole_kernel(const TX* __r
   __shared__ Cand list_s[BW_LIST], best_s[BW_WAVES];
   __shared__ double part_s[BW_WAVES];
   __shared__ float part_m[BW_WAVES];
-  __shared__ uint32_t low_s[64], most_s;
+  __shared__ uint32_t low_s[64], most_s, lanes_s;
   __shared__ int cnt_s, rank_s[BW_LIST];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, b = blockIdx.x;
   const bool busy = wave < N * pieces;             // (the same for the whole wave, like row, at, c, ended, dead)
@@ -420,17 +420,17 @@ __global__ __launch_bounds__(64 * BW_WAVES) void beam_whole_kernel(const TX* __r
     val[i] = v < V ? (float)x[v] : -INFINITY;
   }
   const float c = cum[(int64_t)b * N + row];
-  const bool ended = finished && finished[(int64_t)b * N + row], dead = !(c > -INFINITY);
+  const bool dead = !(c > -INFINITY), ended = finished && finished[(int64_t)b * N + row] && !dead;
   rank_s[tid] = 0;
   if (tid == 0) {
     cnt_s = 0;
-    most_s = 0;
+    most_s = lanes_s = 0;
   }
   // An ended row is one of a single word, a dead one of none.  The word changes places with word 0: it is the first logit of the row's first lane.
   if (dead || ended) {
 #pragma unroll
     for (int i = 0; i < BW_EPT; ++i) val[i] = -INFINITY;
-    if (!dead && at + lane == 0) val[0] = 0.f;
+    if (ended && at + lane == 0) val[0] = 0.f;
   }
   auto word = [&](int i) {
     const int v = at + i * 64 + lane;
@@ -479,13 +479,13 @@ __global__ __launch_bounds__(64 * BW_WAVES) void beam_whole_kernel(const TX* __r
   low = max(wave_group_bound(group, most), most_s);
   if (low <= 0x7fffffu && 4 * N * pieces >= K) low = wave_kth32(group, K);
   if (low <= 0x7fffffu) {                          // (-inf's form; the same for all waves)
-    low = wave_kth32(mine, K);
-    if (lane == 0) atomicMax(&most_s, low);
+    low = wave_kth32(mine, K);                     // (not into most_s: a wave behind this one still has to decide by it)
+    if (lane == 0) atomicMax(&lanes_s, low);
     __syncthreads();
-    low = most_s;
+    low = lanes_s;
   }
   // (read once more: taking it from the registers is a choice among all of them)
-  auto logit = [&](int i) { return dead || ended ? (!dead && at + lane + i == 0 ? 0.f : -INFINITY) : clean((float)x[at + i * 64 + lane]); };
+  auto logit = [&](int i) { return dead || ended ? (ended && at + lane + i == 0 ? 0.f : -INFINITY) : clean((float)x[at + i * 64 + lane]); };
   auto list = [&](uint32_t mask) {
     int to = 0;
     if (mask) to = atomicAdd(&cnt_s, __popc(mask));
