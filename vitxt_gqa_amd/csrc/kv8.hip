@@ -858,9 +858,13 @@ extern "C" int t2s_kv8_attn_splits(int B, int N, int H, int G, int max_tokens, i
   int groups;
   attn_row_tiles(N * G, dtype, &groups);
   const int64_t pairs = (int64_t)B * H * groups;
-  // Few pairs: as many shares as three workgroups to a CU, of 8 blocks (two to a wave) at least.  Many pairs: shares of 20 blocks, so that
+  // Else, few pairs: as many shares as three workgroups to a CU, of 8 blocks (two to a wave) at least.  Many pairs: shares of 20 blocks, so that
   // short sequences leave no long ones to wait for.  Measured, us (5 rows, 10 120 tokens): 12 pairs 1 share 37, 20 shares 9.9, 64 13.7; 96 pairs
   // 1 share 37, 8 15.2, 32 17.7; 768 pairs of ragged lengths 1 share 113, 8 103, 32 120.
+  // Short caches: one share, whose workgroups write the output themselves.  Measured, us with one share and with two and a join (and a launch less, 4 us of the
+  // host's): 12 pairs, 5 rows, bf16, 1 020 tokens 6.9 and 8.4, 1 530 8.5 and 8.4, 2 040 10.0 and 8.5; 192 pairs, 1 530 tokens 9.8 and 13.3; 768 pairs 26 and 30;
+  // fp32, 12 pairs, 1 020 tokens 8.9 and 9.6, 1 530 11.3 and 9.6.
+  if (N * G <= DIRECT_ROWS && blocks <= (dtype == T2S_BF16 ? 24 : 16)) return 1;
   const int64_t s = 768 / pairs >= 2 ? std::min((int64_t)768 / pairs, (int64_t)(blocks + 7) / 8) : (int64_t)(blocks + 19) / 20;
   return (int)(s < 1 ? 1 : s);
 }
