@@ -265,7 +265,7 @@ def test_attend_views():
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("lens,N,H,G,T", [
     ([300, 65], 40, 1, 1, 3), ([640, 1], 1, 1, 48, 20), ([200], 8, 2, 8, 0), ([129], 64, 1, 1, 33), ([500, 0], 65, 1, 1, 2), ([70], 9, 1, 16, 16), ([1500], 6, 1, 5, 0), ([40], 2, 1, 4, 17),
-    ([40], 3, 1, 3, 17), ([1400], 43, 1, 3, 1)])
+    ([40], 3, 1, 3, 17), ([1400], 43, 1, 3, 1), ([3000, 700], 5, 2, 1, 12), ([2600], 1, 2, 4, 0), ([1537, 1536, 1], 3, 1, 1, 5), ([1025, 1024], 2, 1, 2, 1), ([5000], 8, 3, 1, 40)])
 def test_attend_row_groups(dtype, lens, N, H, G, T):
     """One to four 16-row tiles to a group and several groups, with a short cache (a single share) and a longer one, tails on either side of
     what a single share takes in."""
