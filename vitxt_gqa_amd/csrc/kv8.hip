@@ -247,7 +247,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
       __syncthreads();
 #pragma unroll
       for (int w = 0; w < 2; ++w) ((uint4*)(a.codes[w] + (base + blk) * KV_BYTES))[tid] = ((const uint4*)img[w])[tid];
-      // (the next round's barrier behind `red` keeps its image writes behind this round's reads)
+      // (the next block's barrier behind `red` keeps its image writes behind this block's reads)
     }
   }
   if (idle) {
