@@ -9,8 +9,8 @@ Mirrors, with the reference's quirks kept (they change the numbers):
                                  (gt span, predicted frame) pair, a 0 only if the LAST checked pair failed, so the
                                  denominator is the number of appended scores, not of questions)
 * metric wrappers ``stvqa_anls`` / ``IOU@t`` pythia/modules/metrics.py:224-339: the decoding of ``pos_scores`` into answer
-  strings (argmax, OCR-copy indices >= vocabulary size, stop at EOS) and the per-question grounding entries.  The
-  reference reads the grounding annotation from a hard-coded .npy path; here it is handed to the constructor.
+  strings (argmax - or the best beam where there was a beam search -, OCR-copy indices >= vocabulary size, stop at EOS) and the
+  per-question grounding entries.  The reference reads the grounding annotation from a hard-coded .npy path; here it is handed to the constructor.
 * ``EvalAIAnswerProcessor`` / ``TextVQAAccuracyEvaluator`` / ``STVQAAccuracyEvaluator`` :5-274 and the ``textvqa_accuracy``
   wrapper metrics.py:175-222: the VQA-challenge answer normalisation (lower-case, punctuation, number words, articles,
   contractions) and the leave-one-out soft accuracy over 10 human answers.  The contraction table is generated from its
@@ -204,6 +204,14 @@ class STVQAAccuracyEvaluator:
 
 
 # ---- metric wrappers over (sample_list, model_output) ----------------------------------------------------------------
+def answer_inds(model_output):
+    """Indices [B, T] of the answers of an output: the best beam's words where it holds beams (``T2S.set_decoding``), else the largest of each step's
+    ``pos_scores`` (metrics.py:193).  Along a beam the two differ: a step's scores say what would follow the words before it, the beam need not take the largest."""
+    if "beam_tokens" in model_output:
+        return model_output["beam_tokens"][:, 0]
+    return model_output["pos_scores"].argmax(dim=-1)
+
+
 def decode_answers(pred_inds, context_tokens, answer_vocab, vocab_size, eos_idx, word_tokenize=lambda w: w):
     """Indices [B, T] -> answer strings: ids >= vocab_size copy OCR token ``id - vocab_size``; decoding stops at EOS;
     words joined by spaces with " 's" glued back (metrics.py:196-213)."""
@@ -222,7 +230,7 @@ def decode_answers(pred_inds, context_tokens, answer_vocab, vocab_size, eos_idx,
 
 
 class TextVQAAccuracy:
-    """``textvqa_accuracy`` (metrics.py:175-222): decode ``pos_scores`` and score against the 10 human answers."""
+    """``textvqa_accuracy`` (metrics.py:175-222): decode the answers (``answer_inds``) and score against the 10 human answers."""
     name = "textvqa_accuracy"
 
     def __init__(self, answer_vocab, eos_idx, word_tokenize=lambda w: w):
@@ -230,7 +238,7 @@ class TextVQAAccuracy:
         self.evaluator = TextVQAAccuracyEvaluator()
 
     def calculate(self, sample_list, model_output):
-        pred = model_output["pos_scores"].argmax(dim=-1)
+        pred = answer_inds(model_output)
         answers = decode_answers(pred, sample_list["context_tokens"], self.vocab, len(self.vocab), self.eos, self.tok)
         entries = [{"pred_answer": a, "gt_answers": g} for a, g in zip(answers, sample_list["gt_answers"])]
         _, acc = self.evaluator.eval_pred_list([], entries)
@@ -316,7 +324,7 @@ class _RegistryAnswerMetric:
         from .registry import registry
         ap = registry.get(sample_list["dataset_name"] + "_answer_processor")
         vocab_size = ap.get_true_vocab_size()
-        pred = model_output["pos_scores"].argmax(dim=-1)
+        pred = answer_inds(model_output)
         tokens = _batch_objects(sample_list, "context_tokens_enc", "context_tokens")
         gts = _batch_objects(sample_list, "gt_answers_enc", "gt_answers")
         tok = getattr(ap, "word_tokenize", None) or (lambda w: w)

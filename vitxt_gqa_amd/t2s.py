@@ -513,7 +513,7 @@ class T2S(BaseModel):
         over the summed log-softmax of ``pos_scores``; ``beams`` > 1 without a ``cache``: "int8".  A beam ends at the answer processor's ``EOS_IDX``
         if it has one (from there on it repeats that word; the greedy loop goes on); one beam takes the greedy loop's words up to there.  The output
         dict then also holds ``beam_tokens`` [B, beams, D] and ``beam_scores`` [B, beams], best first, and the three passes' scores are those along the
-        best beam."""
+        best beam.  The answer is ``beam_tokens[:, 0]`` (what the answer metrics score), not the argmax of ``pos_scores``: a beam need not take it."""
         if not 1 <= int(beams) <= 16:
             raise ValueError("set_decoding: 1 to 16 beams, got %s" % (beams,))           # (the pointer kernel takes 16 rows a sample)
         if cache is None and beams > 1:
