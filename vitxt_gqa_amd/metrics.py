@@ -206,7 +206,7 @@ class STVQAAccuracyEvaluator:
 # ---- metric wrappers over (sample_list, model_output) ----------------------------------------------------------------
 def answer_inds(model_output):
     """Indices [B, T] of the answers of an output: the best beam's words where it holds beams (``T2S.set_decoding``), else the largest of each step's
-    ``pos_scores`` (metrics.py:193).  Along a beam the two differ: a step's scores say what would follow the words before it, the beam need not take the largest."""
+    ``pos_scores`` (metrics.py:175-222).  Along a beam the two differ: a step's scores say what would follow the words before it, the beam need not take the largest."""
     if "beam_tokens" in model_output:
         return model_output["beam_tokens"][:, 0]
     return model_output["pos_scores"].argmax(dim=-1)
