@@ -45,19 +45,18 @@ __device__ __forceinline__ float from_ordered(uint32_t k) {
 // NaN counts as a masked word, +inf as the largest number
 __device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, 3.402823466e38f); }
 
-// VEC consecutive logits of a row from x[v] on, x + v at a 16-byte boundary; before the row's start and past its end: -inf
+// VEC consecutive logits of a row (16 bytes) from x[v] on; past its end: -inf.  A row may start at any element: the card takes 16 bytes in one load
+// from there as well.
 template <typename TX, int VEC>
-__device__ __forceinline__ void load_logits(const TX* __restrict__ x, int64_t v, int V, float* o) {
-  if (v >= 0 && v + VEC <= V) {
+__device__ __forceinline__ void load_logits(const TX* __restrict__ x, uint32_t v, uint32_t V, float* o) {
+  typedef TX Piece __attribute__((ext_vector_type(VEC), aligned(sizeof(TX))));
+  if (v + VEC <= V) {
+    const Piece f = *(const Piece*)(x + v);
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      const f32x4 f = Vec4<TX>::load(x + v + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i + j] = f[j];
-    }
+    for (int i = 0; i < VEC; ++i) o[i] = (float)f[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = v + i >= 0 && v + i < V ? (float)x[v + i] : -INFINITY;
+    for (int i = 0; i < VEC; ++i) o[i] = v + i < V ? (float)x[v + i] : -INFINITY;
   }
 }
 
@@ -91,17 +90,17 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
   const int64_t row = blockIdx.x / chunks;
   const int b = (int)(row / N), n = (int)(row % N);
   const TX* x = logits + (int64_t)b * l_bs + (int64_t)n * l_ns;
-  // stretches begin at 16-byte boundaries: `skew` elements before the row's first one
-  const int skew = (int)((uintptr_t)x % 16 / sizeof(TX));
+  // (Stretches begin at the row's first element, not at a 16-byte boundary: which logits a lane sums must not depend on where the row lies, or rows of the
+  // same logits would differ in the last bit of their sums, and equal beams would no longer tie.)
   // the first logits are on their way before it is known whether the row's are wanted at all
   float val[BS_EPT];
 #pragma unroll
-  for (int i = 0; i < BS_EPT; i += VEC) load_logits<TX, VEC>(x, (int64_t)chunk * subs * BS_SUB - skew + i * 256 + tid * VEC, V, val + i);
+  for (int i = 0; i < BS_EPT; i += VEC) load_logits<TX, VEC>(x, (uint32_t)(chunk * subs) * BS_SUB + i * 256 + tid * VEC, V, val + i);
   const float c = cum[row];
   const bool dead = !(c > -INFINITY);                                  // -inf or NaN: every candidate of the row is -inf
   const bool ended = finished && finished[row];
   const int64_t out_at = row * chunks + chunk;
-  auto key_of = [](float x, int64_t v) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - (uint32_t)v); };
+  auto key_of = [](float x, uint32_t v) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - v); };
   if (dead || ended) {
     // nothing of the row's logits counts: an ended row offers `pad` at its own score; all else is at -inf, the lowest words first
     if (tid < K) {
@@ -119,8 +118,8 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
   float m = -INFINITY;
   double sum = 0.0;
   for (int sub = chunk * subs; sub < (chunk + 1) * subs; ++sub) {
-    const int64_t v0 = (int64_t)sub * BS_SUB - skew;
-    if (v0 >= V) break;
+    const uint32_t v0 = (uint32_t)sub * BS_SUB;                         // (up to a stretch past V: below 2^32)
+    if (v0 >= (uint32_t)V) break;
     if (sub != chunk * subs)
 #pragma unroll
       for (int i = 0; i < BS_EPT; i += VEC) load_logits<TX, VEC>(x, v0 + i * 256 + tid * VEC, V, val + i);
@@ -148,7 +147,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     // ---- the K best of (this stretch, what is kept of the former ones).  A number that K lanes' best logits reach bounds the K-th largest from
     // below: the least of the maxima of G >= K lane groups of the workgroup (in a row's last stretch, where waves may be without logits, of a wave, and the
     // largest of the four waves' numbers), or the K-th of what is kept already.  That leaves little more than K logits to rank.
-    const bool whole = v0 + BS_SUB <= V;
+    const bool whole = v0 + BS_SUB <= (uint32_t)V;
     __syncthreads();
     const uint64_t kept = tid < K ? top_s[tid] : 0;
     const uint32_t low = wave_group_bound(ordered(mx), whole ? 6 - max(lg - 2, 0) : 6 - lg);
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
     // of one key a lane, at most K (BS_EPT + 1); those are unique.
     uint64_t thr = 1;
     if (cnt > BS_LIST) {
-      int at = index(0) < 0 ? (int)-index(0) : 0;                       // the lane's best: the first that is of the row, or a larger one
+      int at = 0;                                                       // the lane's best: its first logit, or a larger one
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < BS_EPT; ++i)
@@ -179,14 +178,14 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
           top = val[i];
           at = i;
         }
-      const int64_t v_at = v0 + (at / VEC) * VEC * 256 + tid * VEC + at % VEC;
-      const uint64_t best = v_at < V ? key_of(top, v_at) : 0;
+      const uint32_t v_at = v0 + (at / VEC) * VEC * 256 + tid * VEC + at % VEC;
+      const uint64_t best = v_at < (uint32_t)V ? key_of(top, v_at) : 0;
       thr = wave_kth(kept > best ? kept : best, K, 0);
       cnt = __popcll(__ballot(kept >= thr));
       mask = 0;
 #pragma unroll
       for (int i = 0; i < BS_EPT; ++i) {
-        const bool in = index(i) >= 0 && index(i) < V && key_of(val[i], index(i)) >= thr;
+        const bool in = index(i) < (uint32_t)V && key_of(val[i], index(i)) >= thr;
         cnt += __popcll(__ballot(in));
         mask |= in ? 1u << i : 0u;
       }
@@ -205,8 +204,8 @@ __global__ __launch_bounds__(256) void beam_rows_kernel(const TX* __restrict__ l
       float x = val[0];
 #pragma unroll
       for (int j = 1; j < BS_EPT; ++j) x = i == j ? val[j] : x;
-      const int64_t v = v0 + (i / VEC) * VEC * 256 + tid * VEC + i % VEC;
-      if (mask) list_s[to + __popcll(who & ((1ull << lane) - 1))] = v >= 0 && v < V ? key_of(x, v) : 0;
+      const uint32_t v = v0 + (i / VEC) * VEC * 256 + tid * VEC + i % VEC;
+      if (mask) list_s[to + __popcll(who & ((1ull << lane) - 1))] = v < (uint32_t)V ? key_of(x, v) : 0;
       mask &= mask - 1;
       to += __popcll(who);
     }
@@ -666,12 +665,8 @@ int beam_pieces(int64_t N, int64_t V) {
 
 extern "C" int64_t t2s_beam_select_workspace_bytes(int B, int N, int V, int n_select) {
   if (B <= 0 || N <= 0 || V <= 0 || n_select <= 0 || beam_pieces(N, V)) return 0;
-  int chunks = 0, subs;
-  for (int skew : {0, 3, 7}) {                     // (more words may make fewer workgroups of more stretches)
-    int c;
-    beam_chunks((int64_t)B * N, (int64_t)V + skew, &c, &subs);
-    chunks = std::max(chunks, c);
-  }
+  int chunks, subs;
+  beam_chunks((int64_t)B * N, V, &chunks, &subs);
   return (int64_t)B * N * chunks * (8 * (int64_t)n_select + 8 + 4);
 }
 
@@ -698,10 +693,8 @@ extern "C" int t2s_beam_select(const void* logits, int64_t batch_stride, int64_t
     T2S_CHECK_LAUNCH("beam_select");
     return 0;
   }
-  const int64_t es = dtype == T2S_F32 ? 4 : 2;
-  const bool whole = (uintptr_t)logits % 16 == 0 && batch_stride * es % 16 == 0 && beam_stride * es % 16 == 0;
   int chunks, subs;
-  beam_chunks((int64_t)B * N, whole ? V : (int64_t)V + 16 / es - 1, &chunks, &subs);
+  beam_chunks((int64_t)B * N, V, &chunks, &subs);
   const int64_t rows = (int64_t)B * N, grid = rows * chunks;
   T2S_CHECK_ARG(grid < ((int64_t)1 << 24), "beam_select: too many rows");
   uint64_t* keys = (uint64_t*)workspace;
