@@ -10,8 +10,12 @@
 // Selection reads the logits once.  A candidate is a 64-bit key, (logit in an order-preserving integer form) << 32 | ~index: keys are
 // unique, so "descending, ties to the lowest index" is plain integer order, and there is no tie to handle anywhere.  A workgroup
 // holds a stretch of a row in registers, keeps its running maximum / sum of exponentials and its `select` best keys; a second kernel
-// joins the stretches of a sequence and orders the candidates of its N rows by their scores in 64 bits (rows differ by
-// cum - log-sum-exp, which 32 bits would merge into false ties).  Sequences of few logits are one workgroup's, in one launch (below).
+// joins the stretches of a sequence and orders the candidates of its N rows by their scores, compared in 64 bits (in 32, cum - log-sum-exp
+// plus different logits of a row would often round to one number: a false tie).  A row's log-sum-exp itself has fp32's accuracy: 64-bit sums of 16 to 32
+// exponentials each that were made and summed in fp32, within 160 2^-24 of the exact one (terms e^d: 2 |d| + 2 halves of a step, |d| no more than log V
+// on their weighted average; 31 for a lane's sum, 2 for the logarithm).  It is the same number for all candidates of a row and for all rows of the
+// same logits in a call, so nothing within a row and no tie of equal beams depends on it; candidates of unequal beams that are closer than that come in either
+// order.  Sequences of few logits are one workgroup's, in one launch (below).
 //
 // Latencies bound all of it at a beam search's sizes: a stretch of 4 096 logits takes a workgroup 4 us on its own (its logits 2 500 cycles, maxima and
 // sums 600, the bound 800, listing 2 300, ranking 1 500).  Rows and join, us: 64 x 5 x 15 000
@@ -266,7 +270,7 @@ __device__ __forceinline__ uint64_t ordered64(double x) {
 }
 __device__ __forceinline__ double from_ordered64(uint64_t k) { return __builtin_bit_cast(double, k >> 63 ? k ^ 1ull << 63 : ~k); }
 
-// log s of a normal s > 0, off by 2^-24 at most (the exponentials in s are off by as much), 0 for 1: the 64-bit function takes a workgroup a microsecond
+// log s of a normal s > 0, off by 2^-23 at most (s has fp32's accuracy, see above), 0 for 1: the 64-bit function takes a workgroup a microsecond
 __device__ __forceinline__ double log_of(double s) {
   return ((double)__builtin_amdgcn_frexp_exp(s) + (double)__builtin_amdgcn_logf((float)__builtin_amdgcn_frexp_mant(s))) * 0.69314718055994531;
 }
