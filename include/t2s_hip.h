@@ -406,7 +406,7 @@ int t2s_kv8_attn(const void* q, int64_t q_batch_stride, int64_t q_row_stride, in
  *   finished [B, N] bytes or NULL: a beam that has ended offers `pad` at its own score and nothing else (its logits do not count).
  *   Candidates at -inf are taken, lowest first, only when there are no others.  Scores are compared in 64 bits
  *   (different logits of a beam whose scores are one number there - beside one of 1e16 - come in either order).  A row's log sum exp has fp32's
- *   accuracy (off by 160 2^-24 at most) and depends on the row's logits, not on its address or the other rows: beams of equal logits and scores tie;
+ *   accuracy (off by 160 2^-24 at most) and depends on the row's logits and the call's shape, not on an address or other rows: beams of equal logits and scores tie;
  *   candidates of other beams that are closer than that come in either order.
  *   N and n_select at most T2S_BEAM_MAX.  workspace: 8-byte aligned, t2s_beam_select_workspace_bytes (NULL where that is 0),
  *   contents on entry irrelevant.

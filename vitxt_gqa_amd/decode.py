@@ -278,7 +278,7 @@ def beam_select(logits, scores, n_select, finished=None, pad=0):
     ``finished`` bool [B, N]: a beam that has ended offers the token ``pad`` at its own score and nothing else.  NaN logits count as -inf, +inf as
     the largest number.  Returns (scores [B, n_select] float32, parents int64: the beam n, tokens int64: the word v), best first by scores compared in 64 bits, ties
     to the lowest n V + v; candidates at -inf only where nothing else is left.  A row's logsumexp has fp32's accuracy (off by 160 2^-24 = 1e-5 at most) and
-    depends on the row's logits, not on its address or the other rows: beams of equal logits and scores tie, candidates of other beams that are closer than
+    depends on the row's logits and the call's shape, not on an address or other rows: beams of equal logits and scores tie, candidates of other beams that are closer than
     that come in either order.  At most 32 beams and 32 candidates."""
     K, pad, fp = int(n_select), int(pad), None
     if finished is None:
