@@ -19,8 +19,8 @@
 //
 // Latencies bound all of it at a beam search's sizes: a stretch of 4 096 logits takes a workgroup 4 us on its own (its logits 2 500 cycles, maxima and
 // sums 600, the bound 800, listing 2 300, ranking 1 500).  Rows and join, us: 64 x 5 x 15 000
-// fp32 11.5 + 5.1 (15.4 MB), 48 x 8 x 30 522 bf16 16.4 + 7.0 (21.1 MB).  Requesting the next stretch's logits while one is worked on costs a CU one of
-// its six workgroups: 19.5 instead of 16.4.
+// fp32 11.4 + 4.6 (15.4 MB), 48 x 8 x 30 522 bf16 16.1 + 6.8 (21.1 MB).  Requesting the next stretch's logits while one is worked on costs a CU one of
+// its six workgroups: 19.5 where the rows then took 16.4.
 #include <algorithm>
 
 #include "common.h"
@@ -658,8 +658,8 @@ void beam_chunks(int64_t rows, int64_t V, int* chunks, int* subs) {
 }
 
 // Waves of a row where a sequence is a workgroup's, 0 where it has too many logits for one.  Measured, us, one workgroup and rows + join (and a launch
-// less, 3 us of the host's): 1 x 5 beams of 5 600 logits 7.2 and 5.7 + 3.6, 64 of them 8.6 and 7.7 + 4.5, 1 024 35.3 and 34.9 + 4.8; 64 x 16 x 2 048 9.0 and
-// 13.8 + 5.0; 8 x 1 x 32 768, 32 best 9.5 and 13.6 + 8.0; 1 x 1 x 50 5.2 and 4.2 + 2.9.  All logits equal: 31 and 31 + 4.4.
+// less, 3 us of the host's): 1 x 5 beams of 5 600 logits 7.4 and 5.9 + 3.3, 64 of them 9.7 and 7.4 + 4.4, 1 024 37.0 and 31.9 + 4.6; 64 x 16 x 2 048 12.7 and
+// 11.5 + 4.6; 8 x 1 x 32 768, 32 best 9.7 and 8.6 + 8.1; 1 x 1 x 50 5.2 and 4.1 + 2.7.  All of 1 x 5 x 5 600 logits equal: 31 and 31 + 4.7.
 int beam_pieces(int64_t N, int64_t V) {
   const int64_t pieces = (V + BW_PIECE - 1) / BW_PIECE;
   return N * pieces <= BW_WAVES ? (int)pieces : 0;
